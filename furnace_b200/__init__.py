@@ -47,7 +47,8 @@ EXPORTS = [
     "fz_generate", "fz_tokenizer_from_gguf", "fz_tokenizer_new", "fz_tokenizer_free", "fz_tokenizer_vocab_size",
     "fz_tokenizer_encode", "fz_tokenizer_decode", "fz_tokenizer_token_bytes", "fz_pretokenize", "fz_chat_template",
     "fz_utf8_stream_new", "fz_utf8_stream_free", "fz_utf8_stream_push", "fz_utf8_stream_flush",
-    "fz_selftest_exchange_timeout",
+    "fz_selftest_exchange_timeout", "fz_kvq8_append_dev", "fz_kvq8_attend_dev", "fz_kvq8_attend_work",
+    "fz_kvq8_read_dev", "fz_kvq8_status",
 ]
 
 OPS = ["embed", "qkv", "rope_append", "attention", "o_proj", "gate_up", "down", "lm_head", "finalize"]
@@ -68,6 +69,16 @@ class _Config(C.Structure):
 class _TpSlice(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("q_head0", "q_heads", "kv_head0", "kv_heads", "o_col0", "o_cols", "ffn0",
                                           "ffn_n", "vocab0", "vocab_n", "vocab_pad")]
+
+
+class _KvQ8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "rope", "status")] + [
+        (n, C.c_uint32) for n in ("n_pages", "n_rope", "n_heads", "n_kv_heads", "head_dim")]
+
+
+class _KvQ8Seqs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("pages", "lens", "starts")] + [
+        (n, C.c_uint32) for n in ("n_seqs", "max_pages", "max_new", "n_rows")]
 
 
 class _TensorInfo(C.Structure):
@@ -132,6 +143,11 @@ def load_library(build_if_missing: bool = True):
         "fz_weight_free": (None, [P]),
         "fz_matmul_quant_dev": (I, [P, P, U32, P, P]),
         "fz_dequant_dev_noalloc": (I, [U32, P, S, S, P, P]),
+        "fz_kvq8_append_dev": (I, [P, P, U32, P, P, U64, P]),
+        "fz_kvq8_attend_dev": (I, [P, P, U32, P, U64, P, U64, U32, U32, C.c_float, P, U64, P]),
+        "fz_kvq8_attend_work": (I, [P, P, C.POINTER(U64)]),
+        "fz_kvq8_read_dev": (I, [P, P, U32, P, P, U64, P]),
+        "fz_kvq8_status": (I, [P, P]),
         "fz_tp_slice_of": (I, [P, I, I, P]),
         "fz_tp_unique_id": (I, [P, S]),
         "fz_model_load_tp": (I, [P, I, I, P, S, I, pp]),
@@ -453,6 +469,69 @@ class KvCache:
         out = np.zeros((n, kvh * c.head_dim), np.float32)
         _check(load_library().fz_kv_read(self._h, layer, int(which_v), n, _fp(out)))
         return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit paged KV cache on device buffers
+# ---------------------------------------------------------------------------
+KVQ8_PAGE, KVQ8_BLOCK = 64, 16  # positions of a page, positions that share a scale
+
+
+class KvQ8Seqs:
+    """The sequences of a call (fz_kvq8_seqs): device addresses of the page
+    table [n_seqs, max_pages], the lengths [n_seqs] and, unless every sequence
+    has max_new rows, the row starts [n_seqs + 1], all int32.  The caller keeps
+    the buffers alive."""
+
+    def __init__(self, pages: int, lens: int, n_seqs: int, max_pages: int, n_rows: int, starts: int | None = None,
+                 max_new: int = 1):
+        self._s = _KvQ8Seqs(pages, lens, starts, n_seqs, max_pages, max_new, n_rows)
+        self._p = C.addressof(self._s)
+
+
+class KvQ8:
+    """One layer's 8-bit paged KV cache in the caller's device memory
+    (fz_kvq8): device addresses of the codes (page_bytes each page), the f32
+    scales [n_pages, n_kv_heads, 2, 4], one status word (zero at first) and
+    the f32 rotation factors [n_rope, head_dim / 2, 2] (None: no rotation).
+    Calls queue work on `stream` (a cudaStream_t as an int) and return."""
+
+    def __init__(self, codes: int, scales: int, status: int, n_pages: int, n_heads: int, n_kv_heads: int,
+                 head_dim: int, rope: int | None = None, n_rope: int = 0):
+        self._c = _KvQ8(codes, scales, rope, status, n_pages, n_rope, n_heads, n_kv_heads, head_dim)
+        self._p = C.addressof(self._c)
+        self._l = load_library()
+
+    @staticmethod
+    def page_bytes(n_kv_heads: int, head_dim: int) -> int:
+        """Bytes of one page's codes."""
+        return n_kv_heads * 2 * KVQ8_PAGE * head_dim
+
+    def append(self, seqs: KvQ8Seqs, k: int, v: int, ld: int, dtype: int = F32, stream: int = 0):
+        """The call's rows of k (rotated) and v into the cache (fz_kvq8_append_dev)."""
+        _check(self._l.fz_kvq8_append_dev(self._p, seqs._p, dtype, k, v, ld, stream))
+
+    def attend_work(self, seqs: KvQ8Seqs) -> int:
+        """Bytes of device scratch that attend needs."""
+        n = C.c_uint64()
+        _check(self._l.fz_kvq8_attend_work(self._p, seqs._p, C.byref(n)))
+        return n.value
+
+    def attend(self, seqs: KvQ8Seqs, q: int, out: int, ldq: int, ldo: int, work: int, work_bytes: int,
+               dtype: int = F32, window: int = 0, sinks: int = 0, scale: float = 0.0, stream: int = 0):
+        """Attention of the call's rows over the cache, which holds their
+        positions already (fz_kvq8_attend_dev)."""
+        _check(self._l.fz_kvq8_attend_dev(self._p, seqs._p, dtype, q, ldq, out, ldo, window, sinks, scale, work,
+                                          work_bytes, stream))
+
+    def read(self, seqs: KvQ8Seqs, k: int | None, v: int | None, ld: int, dtype: int = F32, stream: int = 0):
+        """The call's rows as the cache holds them (fz_kvq8_read_dev)."""
+        _check(self._l.fz_kvq8_read_dev(self._p, seqs._p, dtype, k, v, ld, stream))
+
+    def status(self, stream: int = 0):
+        """Wait for the stream; raise FurnaceError if a kernel found numbers
+        out of range or values that are not finite since the last call."""
+        _check(self._l.fz_kvq8_status(self._p, stream))
 
 
 # ---------------------------------------------------------------------------

@@ -1920,6 +1920,11 @@ void launch_prefill_attention(const float* qkv, uint32_t ldq, const float* rope_
 }
 
 // ---------------------------------------------------------------------------
+// 8-bit paged KV cache
+// ---------------------------------------------------------------------------
+#include "kvq8.cuh"
+
+// ---------------------------------------------------------------------------
 // Sampling support (src/sampler.rs:39-155): repeat penalty, temperature and
 // top-k selection on the device.  Keys (orderable(l / temp) << 32 | ~index)
 // sort descending by value and ascending by index on ties, the order of the

@@ -170,4 +170,40 @@ void launch_prefill_attention(const float* qkv, uint32_t ldq, const float* rope_
                               float* ctx, uint32_t ldc, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t max_ctx,
                               uint32_t pos0, uint32_t T, uint32_t* err, cudaStream_t s);
 
+// ---- 8-bit paged KV cache (kvq8.cuh) ------------------------------------------
+// Device view of an fz_kvq8 (include/furnace.h).
+struct KvQ8Dev {
+  uint8_t* codes;
+  float* scales;
+  const float2* rope;  // null: keys and queries are taken as they are
+  uint32_t* status;    // KQ_* bits, set by the kernels
+  uint32_t n_pages, n_rope, nkv, group, hd;
+};
+enum : uint32_t { KQ_BAD_LEN = 1, KQ_BAD_PAGE = 2, KQ_BAD_POS = 4, KQ_NOT_FINITE = 8 };
+// Device view of an fz_kvq8_seqs: sequence i holds lens[i] + len_add positions
+// (lens null: len_add), its last starts[i + 1] - starts[i] (starts null:
+// max_new) are the call's rows; pages null: page j of sequence i is i *
+// max_pages + j.
+struct KvQ8Batch {
+  const int32_t *pages, *lens, *starts;
+  uint32_t n_seqs, max_pages, max_new, n_rows;
+  int32_t len_add;
+};
+struct KvQ8Attend {
+  KvQ8Dev c;
+  KvQ8Batch b;
+  bool f16;  // q and out elements
+  const void* q;
+  void* out;
+  uint64_t ldq, ldo;
+  uint32_t window, sinks;
+  float scale;
+  void* work;  // kvq8_attend_work(c, b) bytes
+};
+void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const void* k, const void* v, uint64_t ld,
+                        cudaStream_t s);
+void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, void* v, uint64_t ld, cudaStream_t s);
+uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b);
+void launch_kvq8_attend(const KvQ8Attend& a, cudaStream_t s);
+
 }  // namespace fz

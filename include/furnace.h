@@ -311,6 +311,94 @@ int fz_matmul_quant_dev(const fz_weight* w, const float* a_dev, uint32_t seq, fl
 int fz_dequant_dev_noalloc(uint32_t dtype, const void* raw_dev, size_t nbytes, size_t n, float* out_dev,
                            void* stream);
 
+/* ---- 8-bit paged KV cache on device buffers --------------------------------
+ * No counterpart in the reference, whose cache is one f32 row per position
+ * (src/model.rs:321-363).  Keys and values of many sequences live in pages of
+ * FZ_KVQ8_PAGE positions that the caller hands out; an element is one byte,
+ * code + 128 with code in [-127, 127], and stands for code * scale, one f32
+ * scale per block of FZ_KVQ8_BLOCK positions, KV head and side (keys, values).
+ * All buffers are the caller's device memory on one device; the calls queue
+ * work on `stream` (a cudaStream_t as void*) of that device, which need not be
+ * the current one, allocate nothing, never synchronise and may be captured
+ * into a graph.
+ *
+ * What only the device can check (lengths, rows, page numbers, positions
+ * beyond the rotation table, values that are not finite) sets bits of
+ * *status: a sequence or page with a bad number is left out of the call, its
+ * outputs are undefined, and nothing outside the buffers is touched.
+ * fz_kvq8_status reports and clears the bits. */
+enum { FZ_KVQ8_PAGE = 64, FZ_KVQ8_BLOCK = 16 };
+
+/* One layer's cache.  codes: n_pages * n_kv_heads * 2 * 64 * head_dim bytes,
+ * 16-byte aligned: page, KV head, side (0 keys, 1 values), 4 blocks.  Inside a
+ * block of 16 positions the byte of position p, dimension d is at
+ *   keys:   (p / 8) * 8 * head_dim + (d / 64) * 512 + (p % 8) * 64 + d % 64
+ *   values: (d / 32) * 512 + (d % 8) * 64 + (p % 8 / 2) * 16 + (d % 32 / 8) * 4
+ *           + (p / 8) * 2 + p % 2
+ * scales: [n_pages][n_kv_heads][2][4] f32.  rope: [n_rope][head_dim / 2][2] f32
+ * (cos, sin) of every position, or NULL with n_rope 0: keys and queries are
+ * then taken as they are.  head_dim is 64 or 128; n_heads (the query heads) a
+ * multiple of n_kv_heads.  Neither codes nor scales need to be initialised. */
+typedef struct fz_kvq8 {
+  void* codes;
+  float* scales;
+  const float* rope;
+  uint32_t* status; /* one word, zero before the first call */
+  uint32_t n_pages, n_rope, n_heads, n_kv_heads, head_dim;
+} fz_kvq8;
+
+/* The sequences of a call.  pages: [n_seqs][max_pages], the page that holds
+ * positions 64 j .. 64 j + 63 of sequence i at pages[i * max_pages + j];
+ * entries past a sequence's last position are not read.  lens: [n_seqs], the
+ * positions each sequence holds, this call's among them; 0 is a sequence
+ * without positions.  starts: [n_seqs + 1], sequence i's last starts[i + 1] -
+ * starts[i] (0 .. max_new) positions are rows starts[i] .. of the call's row
+ * buffers; NULL: every sequence has max_new rows, i * max_new ...  n_rows: the
+ * rows the buffers hold (rows of no sequence are left as they are). */
+typedef struct fz_kvq8_seqs {
+  const int32_t* pages;
+  const int32_t* lens;
+  const int32_t* starts;
+  uint32_t n_seqs, max_pages, max_new, n_rows;
+} fz_kvq8_seqs;
+
+/* Rows of k, v, q and out hold heads back to back (head h at h * head_dim), row
+ * r at r * ld elements; dtype FZ_F32 or FZ_F16.  Pointers and row strides are
+ * multiples of 16 bytes, so that k, v and q may be columns of one q|k|v row. */
+
+/* Append the call's rows: k, rotated at its position (pairs head_dim / 2
+ * apart, a*c - b*s and a*s + b*c in f32, src/model.rs:193-217), and v.  For
+ * every block written, scale = (largest magnitude of the call's values in it)
+ * / 127, and at least the block's scale so far when it keeps older positions;
+ * these then take the codes round(code * (old scale / scale)).  Codes are
+ * round(x / scale), all in f32, rounding to nearest even.  Values must be
+ * finite; one that is not makes the block's scale a NaN (reported).  Two
+ * sequences of a call must not append to the same page. */
+int fz_kvq8_append_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, const void* k, const void* v,
+                       uint64_t ld, void* stream);
+
+/* Attention of the call's rows over the cache, which already holds their
+ * positions (append first): row at position p, query head h sees positions t
+ * <= p of KV head h / (n_heads / n_kv_heads); with a window (0: none) only
+ * those with t > p - window or t < sinks.  q is rotated at p like k.  out =
+ * sum_t softmax(scale * q.k)_t v_t, statistics and sums in f32; scale 0 means
+ * 1 / sqrt(head_dim).  out must not overlap q.  work: device scratch of at
+ * least fz_kvq8_attend_work bytes, 16-byte aligned, contents don't matter;
+ * calls that may run at the same time need one each. */
+int fz_kvq8_attend_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, const void* q, uint64_t ldq,
+                       void* out, uint64_t ldo, uint32_t window, uint32_t sinks, float scale, void* work,
+                       uint64_t work_bytes, void* stream);
+int fz_kvq8_attend_work(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint64_t* bytes);
+
+/* The call's rows as the cache holds them (keys rotated), code * scale; k or
+ * v may be NULL. */
+int fz_kvq8_read_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, void* k, void* v, uint64_t ld,
+                     void* stream);
+
+/* Wait for `stream`, then report what the kernels found in their inputs since
+ * the last report: FZ_EINVAL with a message naming it, FZ_OK if nothing. */
+int fz_kvq8_status(const fz_kvq8* kv, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
