@@ -184,64 +184,489 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 }
 
 // ---------------------------------------------------------------------------
-// Attention: one CTA of four warps per (row, query head); a warp takes every
-// fourth visible position, its lanes the dims, with an online softmax, and
-// the four warps' sums meet in shared memory.
+// Attention of few rows over long caches (k_kvq8_split + k_kvq8_merge).
+//
+// A tile is one page of one KV head for one group of 8 rows (row = (new token,
+// query head of the KV head)).  All tiles of the call, sequence by sequence,
+// are cut into equal runs, one per CTA, so that ragged batches load the SMs
+// evenly; a run may hold several segments ((sequence, KV head, row group)) and
+// a segment may span several runs: it is then written as partial results that
+// k_kvq8_merge joins.
+//
+// The cache bytes bound the kernel, so everything else has to fit under them.
+// One warp takes 16 positions (a block) of the page.  Codes become fp16
+// exactly (0x6400 | byte is 1024 + byte: one byte permute and one subtraction
+// for two of them) and both products run on mma.m16n8k16: its 16 rows are the
+// 8 query rows twice, as the high and the low part of an 11 + 11 bit split, so
+// that the products keep f32's precision at no further cost.  The block's
+// scales stay outside: the keys' multiplies the score, the values' the
+// probability before its split.
+//
+// Softmax: with scores x_t (base 2) and value scales v_t the running maximum m
+// is taken over x_t + log2 v_t.  The weights w_t = 2^(x_t - m) v_t that
+// multiply the codes are then at most 1, whatever the scales, and l = sum
+// 2^(x_t - m) is the denominator.  Scales under 2^-100 count as that in m, so
+// that l stays finite.
 // ---------------------------------------------------------------------------
-constexpr int KQ_AT_THREADS = 128;
+constexpr int KQ_SP_THREADS = 128;
+constexpr uint32_t KQ_SP_STAGES = 4;     // tiles in flight per warp
+constexpr uint32_t KQ_SP_CTAS = 3;       // CTAs per SM
+constexpr float KQ_MIN_SCALE = 7.8886090522101181e-31f;  // 2^-100
+
+template <int HD>
+struct KqSplitSmem {
+  struct Stage {
+    uint8_t k[KQ_BLOCK * HD], v[KQ_BLOCK * HD];
+    float scale[4];  // keys, values
+  };
+  union {
+    Stage ring[KQ_SP_THREADS / 32][KQ_SP_STAGES];
+    float acc[KQ_SP_THREADS / 32][8][HD];  // the warps' sums at a segment's end
+  };
+  __half qh[8][HD], ql[8][HD];
+  float rowf[8];
+  int32_t rowpos[8];
+  float m[KQ_SP_THREADS / 32][8], l[KQ_SP_THREADS / 32][8];
+  uint64_t scan[KQ_SP_THREADS / 32];
+};
+
+// The pages of a sequence that any of its new positions sees: virtual page v
+// is page v below n_sink, lo + v - n_sink from there on; n pages in all.
+struct KqSpan {
+  uint32_t n_sink, lo, n;
+  __device__ __forceinline__ uint32_t page(uint32_t v) const { return v < n_sink ? v : lo + v - n_sink; }
+};
+__device__ __forceinline__ KqSpan kq_span(uint32_t pmin, uint32_t pmax, uint32_t window, uint32_t sinks) {
+  KqSpan r{0, 0, 0};
+  if (window && pmin >= window) {
+    r.lo = (pmin - window + 1) / KQ_PAGE;
+    r.n_sink = min(sinks / KQ_PAGE + (sinks % KQ_PAGE != 0), r.lo);
+  }
+  r.n = r.n_sink + pmax / KQ_PAGE - r.lo + 1;
+  return r;
+}
+
+// What the split form needs to know of a sequence.
+struct KqPlan {
+  KqSeq s;
+  KqSpan span;
+  uint32_t groups;  // row groups of one KV head
+  __device__ __forceinline__ uint64_t tiles(uint32_t nkv) const { return (uint64_t)groups * span.n * nkv; }
+};
+__device__ __forceinline__ KqPlan kq_plan(const KvQ8Dev& c, const KvQ8Batch& b, uint32_t i, uint32_t window,
+                                          uint32_t sinks) {
+  KqPlan p;
+  p.s = kq_seq(b, i, c.status);
+  if (p.s.n_new && c.rope && p.s.len > (int64_t)c.n_rope) {
+    atomicOr(c.status, KQ_BAD_POS);
+    p.s.n_new = 0;
+  }
+  p.groups = ((uint32_t)p.s.n_new * c.group + 7) / 8;
+  p.span = KqSpan{0, 0, 0};
+  if (p.s.n_new) p.span = kq_span(p.s.len - p.s.n_new, p.s.len - 1, window, sinks);
+  return p;
+}
+
+__device__ __forceinline__ void kq_mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four bytes (code + 128) as fp16 codes, exactly.
+__device__ __forceinline__ void kq_halves(uint32_t w, uint32_t* h) {
+  const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1024 + 128
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  h[0] = *reinterpret_cast<const uint32_t*>(&x);
+  h[1] = *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t kq_pack(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// High and low parts of two values: hi = rn(x), lo = rn((x - hi) * 2^11).
+__device__ __forceinline__ void kq_split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = kq_pack((a - f.x) * 2048.f, (b - f.y) * 2048.f);
+}
+__device__ __forceinline__ void kq_cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void kq_cp4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// Partial results: one slot per run end.  A slot holds the 8 rows' sums of
+// codes, then their m, then their l.
+template <int HD>
+__host__ __device__ constexpr uint32_t kq_slot_floats() {
+  return 8 * HD + 16;
+}
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(KQ_AT_THREADS) k_kvq8_attend(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ q,
-                                                               uint64_t ldq, T* __restrict__ out, uint64_t ldo,
-                                                               uint32_t window, uint32_t sinks, float scale) {
+struct KqSplitArgs {
+  KvQ8Dev c;
+  KvQ8Batch b;
+  const T* q;
+  T* out;
+  uint64_t ldq, ldo;
+  uint32_t window, sinks;
+  float scale;          // softmax scale * log2(e)
+  uint64_t* prefix;     // [n_seqs + 1] tiles before each sequence (written by CTA 0)
+  float* slots;         // [2 * gridDim.x]
+};
+
+// Rows of one segment in shared memory: rotated, scaled by a power of two to
+// a largest magnitude in [2^13, 2^14), split.  rowf undoes the power and holds
+// the softmax scale; rowpos is the row's position, -1 for a row that is none.
+template <int HD, typename T>
+__device__ __forceinline__ void kq_load_rows(const KqSplitArgs<HD, T>& a, KqSplitSmem<HD>& sm, const KqSeq& s,
+                                             uint32_t kvh, uint32_t grp) {
+  constexpr uint32_t half = HD / 2, N = half / 16;  // pairs per thread
+  const uint32_t r = threadIdx.x >> 4, l16 = threadIdx.x & 15, rr = grp * 8 + r, j = rr / a.c.group;
+  const bool live = j < (uint32_t)s.n_new;
+  const uint32_t pos = s.len - s.n_new + j;
+  float x[2 * N], top = 0.f;
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) {
+    const uint32_t d = l16 * N + i;
+    float u = 0.f, w = 0.f;
+    if (live) {
+      const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d;
+      u = kq_ld(p);
+      w = kq_ld(p + half);
+      if (a.c.rope) {
+        const float2 f = a.c.rope[(uint64_t)pos * half + d];
+        const float v = __fsub_rn(__fmul_rn(u, f.x), __fmul_rn(w, f.y));
+        w = __fadd_rn(__fmul_rn(u, f.y), __fmul_rn(w, f.x));
+        u = v;
+      }
+    }
+    x[i] = u;
+    x[N + i] = w;
+    top = fmaxf(top, fmaxf(fabsf(u), fabsf(w)));
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+  e = max(e, -100);
+  const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);  // e <= 128: the exponent stays positive
+#pragma unroll
+  for (uint32_t i = 0; i < N; i++) {
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++) {
+      const float v = x[k * N + i] * up;
+      const __half hi = __float2half_rn(v);
+      sm.qh[r][k * half + l16 * N + i] = hi;
+      sm.ql[r][k * half + l16 * N + i] = __float2half_rn((v - __half2float(hi)) * 2048.f);
+    }
+  }
+  if (l16 == 0) {
+    sm.rowf[r] = a.scale * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+    sm.rowpos[r] = live ? (int32_t)pos : -1;
+  }
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const __grid_constant__ KqSplitArgs<HD, T> a) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
+  constexpr uint32_t KJ = HD / 64, NQ = HD / 32;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   pdl_trigger();
   pdl_wait();
-  constexpr int DPL = HD / 32;
-  const KqSeq s = kq_seq(b, blockIdx.z, c.status);
-  if ((int32_t)blockIdx.x >= s.n_new) return;
-  const uint32_t head = blockIdx.y, h = head / c.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t pos = s.len - s.n_new + blockIdx.x, row = s.row0 + blockIdx.x;
-  if (c.rope && pos >= c.n_rope) {
-    if (threadIdx.x == 0) atomicOr(c.status, KQ_BAD_POS);
-    return;
+  // this CTA's run of tiles [w0, w1) and the sequence it starts in
+  uint64_t total = 0;
+  for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
+    const uint32_t i = i0 + tid;
+    uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv) : 0;
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) sm.scan[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < KQ_SP_THREADS / 32; w++) total += sm.scan[w];
+    __syncthreads();
   }
-  float qv[DPL], acc[DPL], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < DPL; i++) {
-    qv[i] = kq_rotated<HD>(q + (uint64_t)row * ldq + (uint64_t)head * HD,
-                           c.rope ? c.rope + (uint64_t)pos * (HD / 2) : nullptr, lane + 32 * i);
-    acc[i] = 0.f;
-  }
-  for (uint32_t t = warp; t <= pos; t += 4) {
-    if (window && pos - t >= window && t >= sinks) continue;
-    const int32_t page = kq_page(c, b, blockIdx.z, t / KQ_PAGE);
-    if (page < 0) continue;
-    const uint32_t sub = t / KQ_BLOCK % KQ_NB, tok = t % KQ_BLOCK;
-    const uint64_t side = ((uint64_t)page * c.nkv + h) * 2;
-    const uint8_t* kc = c.codes + side * KQ_PAGE * HD + sub * KQ_BLOCK * HD;
-    float d = 0.f;
-    for (int i = 0; i < DPL; i++) d = fmaf(qv[i], (float)((int)kc[kq_koff<HD>(tok, lane + 32 * i)] - 128), d);
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    d *= scale * c.scales[side * KQ_NB + sub];
-    const float mn = fmaxf(m, d), alpha = expf(m - mn), p = expf(d - mn);
-    const float pv = p * c.scales[(side + 1) * KQ_NB + sub];
-    l = fmaf(l, alpha, p);
-    m = mn;
-    for (int i = 0; i < DPL; i++)
-      acc[i] = fmaf(acc[i], alpha, pv * (float)((int)kc[KQ_PAGE * HD + kq_voff(tok, lane + 32 * i)] - 128));
-  }
-  __shared__ float sm[4], sl[4], sa[4][HD];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-  for (int i = 0; i < DPL; i++) sa[warp][lane + 32 * i] = acc[i];
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  for (uint32_t d = threadIdx.x; d < HD; d += KQ_AT_THREADS) {
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < 4; w++) {
-      const float f = sm[w] == -INFINITY ? 0.f : expf(sm[w] - top);
-      num = fmaf(f, sa[w][d], num);
-      den = fmaf(f, sl[w], den);
+  const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+  const uint64_t w0 = min(per * blockIdx.x, total), w1 = min(w0 + per, total);
+  uint64_t before = 0, off = 0;
+  uint32_t seq = 0;
+  if (a.b.n_seqs > 1 || blockIdx.x == 0) {
+    __shared__ uint32_t s_seq;
+    __shared__ uint64_t s_off;
+    for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
+      const uint32_t i = i0 + tid;
+      const uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv) : 0;
+      uint64_t inc = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += x;
+      }
+      if (lane == 31) sm.scan[warp] = inc;
+      __syncthreads();
+      uint64_t base = before;
+      for (uint32_t w = 0; w < KQ_SP_THREADS / 32; w++) {
+        if (w < warp) base += sm.scan[w];
+        before += sm.scan[w];
+      }
+      if (blockIdx.x == 0 && i < a.b.n_seqs) a.prefix[i] = base + inc - n;
+      if (n && w0 >= base + inc - n && w0 < base + inc) {
+        s_seq = i;
+        s_off = w0 - (base + inc - n);
+      }
+      __syncthreads();
     }
-    kq_st(out + (uint64_t)row * ldo + (uint64_t)head * HD + d, den == 0.f ? 0.f : __fdiv_rn(num, den));
+    if (blockIdx.x == 0 && tid == 0) a.prefix[a.b.n_seqs] = total;
+    if (w0 < w1) {
+      seq = s_seq;
+      off = s_off;
+    }
+  } else {
+    off = w0;
+  }
+  if (w0 >= w1) return;
+
+  KqPlan p = kq_plan(a.c, a.b, seq, a.window, a.sinks);
+  uint64_t w = w0;
+  while (w < w1) {
+    while (off >= p.tiles(a.c.nkv)) {
+      off -= p.tiles(a.c.nkv);
+      p = kq_plan(a.c, a.b, ++seq, a.window, a.sinks);  // w < total: a later sequence has tiles
+    }
+    const uint32_t seg = (uint32_t)(off / p.span.n), v0 = (uint32_t)(off % p.span.n);
+    const uint32_t nv = (uint32_t)min((uint64_t)(p.span.n - v0), w1 - w);
+    const uint32_t kvh = seg / p.groups, grp = seg % p.groups;
+    const uint32_t j0 = grp * 8 / a.c.group, j1 = min((grp * 8 + 7) / a.c.group, (uint32_t)p.s.n_new - 1);
+    const uint32_t plo = p.s.len - p.s.n_new + j0, phi = p.s.len - p.s.n_new + j1;  // the group's positions
+
+    // pages of the next 32 tiles, one per lane, and of the 32 after them
+    const int32_t last = (int32_t)nv - 1;
+    auto page_of = [&](uint32_t i) { return max(kq_page(a.c, a.b, seq, p.span.page(v0 + min((int32_t)i, last))), 0); };
+    int32_t pid = page_of(lane), pid_next = nv > 32 ? page_of(32 + lane) : 0;
+    uint32_t issued = 0;
+    // the warp's block of tile i, unless none of the group's rows sees it
+    auto block_pos = [&](uint32_t i) { return p.span.page(v0 + i) * KQ_PAGE + warp * KQ_BLOCK; };
+    auto dead = [&](uint32_t pos) {
+      return pos > phi || (a.window && pos + KQ_BLOCK <= plo && plo - (pos + KQ_BLOCK - 1) >= a.window && pos >= a.sinks);
+    };
+    auto issue = [&]() {
+      const uint32_t i = issued++;
+      if (i < nv) {
+        if (i && i % 32 == 0) {
+          pid = pid_next;
+          pid_next = i + 32 < nv ? page_of(i + 32 + lane) : 0;
+        }
+        const int32_t page = __shfl_sync(0xffffffffu, pid, i % 32);
+        if (!dead(block_pos(i))) {
+          auto& st = sm.ring[warp][i % KQ_SP_STAGES];
+          const uint64_t side = ((uint64_t)page * a.c.nkv + kvh) * 2;
+          const uint8_t* src = a.c.codes + side * KQ_PAGE * HD + warp * KQ_BLOCK * HD;
+#pragma unroll
+          for (uint32_t x = 0; x < KQ_BLOCK * HD / 512; x++) {
+            kq_cp16(st.k + x * 512 + lane * 16, src + x * 512 + lane * 16);
+            kq_cp16(st.v + x * 512 + lane * 16, src + KQ_PAGE * HD + x * 512 + lane * 16);
+          }
+          if (lane < 2) kq_cp4(&st.scale[lane], a.c.scales + (side + lane) * KQ_NB + warp);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (uint32_t i = 0; i + 1 < KQ_SP_STAGES; i++) issue();
+
+    kq_load_rows<HD, T>(a, sm, p.s, kvh, grp);
+    __syncthreads();
+    uint32_t qh[KJ][8], ql[KJ][8];  // row g, dims 64j + 16t .. + 15
+#pragma unroll
+    for (uint32_t j = 0; j < KJ; j++)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) {
+        qh[j][i] = *reinterpret_cast<const uint32_t*>(&sm.qh[g][j * 64 + t * 16 + 2 * i]);
+        ql[j][i] = *reinterpret_cast<const uint32_t*>(&sm.ql[g][j * 64 + t * 16 + 2 * i]);
+      }
+    const float rowf = sm.rowf[g];
+    const int32_t rowpos = sm.rowpos[g];
+    float m = -INFINITY, l = 0.f, o[HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < HD / 8; n++)
+#pragma unroll
+      for (int x = 0; x < 4; x++) o[n][x] = 0.f;
+
+    for (uint32_t i = 0; i < nv; i++) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(KQ_SP_STAGES - 2) : "memory");
+      __syncwarp();  // every lane's copies have landed, and every lane is done with the stage refilled next
+      issue();
+      const uint32_t pos = block_pos(i);
+      if (dead(pos)) continue;
+      auto& st = sm.ring[warp][i % KQ_SP_STAGES];
+      float sacc[2][4] = {};
+#pragma unroll
+      for (uint32_t n = 0; n < 2; n++)
+#pragma unroll
+        for (uint32_t j = 0; j < KJ; j++) {
+          const uint4 kw = *reinterpret_cast<const uint4*>(st.k + n * 8 * HD + j * 512 + lane * 16);
+          const uint32_t word[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+          for (uint32_t x = 0; x < 4; x++) {
+            uint32_t h[2];
+            kq_halves(word[x], h);
+            const uint32_t qa[4] = {qh[j][2 * x], ql[j][2 * x], qh[j][2 * x + 1], ql[j][2 * x + 1]};
+            kq_mma(sacc[n], qa, h[0], h[1]);
+          }
+        }
+      const float ks = st.scale[0] * rowf, vs = st.scale[1];
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) x[k] = fmaf(sacc[k >> 1][2 + (k & 1)], 1.f / 2048.f, sacc[k >> 1][k & 1]) * ks;
+      if (!(pos + KQ_BLOCK - 1 <= plo &&
+            (!a.window || pos + KQ_BLOCK - 1 < a.sinks || pos > phi || phi - pos < a.window) && rowpos >= 0)) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int32_t at = (int32_t)pos + (k >> 1) * 8 + 2 * t + (k & 1);
+          const bool seen =
+              at <= rowpos && (!a.window || (uint32_t)(rowpos - at) < a.window || (uint32_t)at < a.sinks);
+          if (!seen) x[k] = -INFINITY;
+        }
+      }
+      float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) + __log2f(fmaxf(vs, KQ_MIN_SCALE));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float mn = fmaxf(m, top), sub = mn == -INFINITY ? 0.f : mn;
+      const float alpha = mn == m ? 1.f : exp2f(m - sub);
+      m = mn;
+      float wv[4], ps = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float e = exp2f(x[k] - sub);
+        ps += e;
+        wv[k] = x[k] == -INFINITY ? 0.f : e * vs;
+      }
+      l = fmaf(l, alpha, ps);
+      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < HD / 8; n++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[n][k] *= alpha;
+      }
+      uint32_t pa[4];
+      kq_split2(wv[0], wv[1], &pa[0], &pa[1]);
+      kq_split2(wv[2], wv[3], &pa[2], &pa[3]);
+#pragma unroll
+      for (uint32_t n = 0; n < NQ; n++) {
+        const uint4 vw = *reinterpret_cast<const uint4*>(st.v + n * 512 + lane * 16);
+        const uint32_t word[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+          uint32_t h[2];
+          kq_halves(word[k], h);
+          kq_mma(o[n * 4 + k], pa, h[0], h[1]);
+        }
+      }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the ring is free
+    if (t == 0) {
+      sm.m[warp][g] = m;
+      sm.l[warp][g] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 8; n++)
+      *reinterpret_cast<float2*>(&sm.acc[warp][g][n * 8 + 2 * t]) =
+          make_float2(fmaf(o[n][2], 1.f / 2048.f, o[n][0]), fmaf(o[n][3], 1.f / 2048.f, o[n][1]));
+    __syncthreads();
+    const bool whole = nv == p.span.n;
+    // a run has at most two pieces that are not whole segments: its first and its last
+    float* slot = a.slots + (2ull * blockIdx.x + (w != w0)) * kq_slot_floats<HD>();
+    for (uint32_t x = tid; x < 8 * HD; x += KQ_SP_THREADS) {
+      const uint32_t r = x / HD, d = x % HD;
+      const float top = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int y = 0; y < KQ_SP_THREADS / 32; y++) {
+        const float f = sm.m[y][r] == -INFINITY ? 0.f : exp2f(sm.m[y][r] - top);
+        num = fmaf(f, sm.acc[y][r][d], num);
+        den = fmaf(f, sm.l[y][r], den);
+      }
+      if (whole) {
+        const uint32_t rr = grp * 8 + r, j = rr / a.c.group;
+        if (j < (uint32_t)p.s.n_new)
+          kq_st(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d,
+                den == 0.f ? 0.f : __fdiv_rn(num, den));
+      } else {
+        slot[x] = num;
+        if (d == 0) {
+          slot[8 * HD + r] = top;
+          slot[8 * HD + 8 + r] = den;
+        }
+      }
+    }
+    __syncthreads();  // shared memory is reused by the next segment
+    w += nv;
+    off += nv;
+  }
+}
+
+// Join the pieces of a segment that spans several runs.  Grid (rows of a KV
+// head, nkv, n_seqs); four warps take every fourth piece, a lane HD / 32 dims.
+constexpr int KQ_MG_THREADS = 128;
+constexpr uint32_t KQ_MG_PIECES = 1024;  // runs of a call at most
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_constant__ KqSplitArgs<HD, T> a,
+                                                              uint32_t runs) {
+  pdl_wait();
+  const KqPlan p = kq_plan(a.c, a.b, blockIdx.z, a.window, a.sinks);
+  const uint32_t rr = blockIdx.x, kvh = blockIdx.y, grp = rr / 8, r = rr % 8, j = rr / a.c.group;
+  if (j >= (uint32_t)p.s.n_new) return;
+  const uint64_t total = a.prefix[a.b.n_seqs], per = (total + runs - 1) / runs;
+  const uint64_t s0 = a.prefix[blockIdx.z] + (uint64_t)(kvh * p.groups + grp) * p.span.n, s1 = s0 + p.span.n;
+  const uint32_t i0 = (uint32_t)(s0 / per), n = (uint32_t)((s1 - 1) / per) - i0 + 1;
+  if (n == 1) return;  // written by the run itself
+  __shared__ float wt[KQ_MG_PIECES];
+  __shared__ float red[KQ_MG_THREADS / 32][HD], rden[KQ_MG_THREADS / 32], rtop[KQ_MG_THREADS / 32];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto slot = [&](uint32_t i) {  // run i0 + i: its first piece unless the segment starts inside it
+    return a.slots + (2ull * (i0 + i) + ((uint64_t)(i0 + i) * per < s0)) * kq_slot_floats<HD>();
+  };
+  float top = -INFINITY;
+  for (uint32_t i = tid; i < n; i += KQ_MG_THREADS) {
+    const float m = slot(i)[8 * HD + r];
+    wt[i] = m;
+    top = fmaxf(top, m);
+  }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) rtop[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(rtop[0], rtop[1]), fmaxf(rtop[2], rtop[3]));
+  float den = 0.f;
+  for (uint32_t i = tid; i < n; i += KQ_MG_THREADS) {
+    const float f = wt[i] == -INFINITY ? 0.f : exp2f(wt[i] - top);
+    wt[i] = f;
+    den = fmaf(f, slot(i)[8 * HD + 8 + r], den);
+  }
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  if (lane == 0) rden[warp] = den;
+  __syncthreads();
+  constexpr int DPL = HD / 32;
+  float acc[DPL] = {};
+#pragma unroll 4
+  for (uint32_t i = warp; i < n; i += KQ_MG_THREADS / 32) {
+    const float* x = slot(i) + r * HD + lane * DPL;
+#pragma unroll
+    for (int d = 0; d < DPL; d++) acc[d] = fmaf(wt[i], x[d], acc[d]);
+  }
+#pragma unroll
+  for (int d = 0; d < DPL; d++) red[warp][lane * DPL + d] = acc[d];
+  __syncthreads();
+  if (tid < HD) {
+    const float num = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+    den = (rden[0] + rden[1]) + (rden[2] + rden[3]);
+    kq_st(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + tid,
+          den == 0.f ? 0.f : __fdiv_rn(num, den));
   }
 }
 
@@ -279,16 +704,36 @@ void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, v
     f16 ? kvq8_read_t<64, __half>(c, b, k, v, ld, s) : kvq8_read_t<64, float>(c, b, k, v, ld, s);
 }
 
+// Runs of the split form: every SM filled, never more than there can be tiles.
+static uint32_t kvq8_runs(const KvQ8Dev& c, const KvQ8Batch& b) {
+  const uint64_t most = (uint64_t)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8) * b.max_pages;
+  return (uint32_t)std::min<uint64_t>({most, (uint64_t)num_sms() * KQ_SP_CTAS, KQ_MG_PIECES});
+}
+static uint64_t kvq8_prefix_bytes(const KvQ8Batch& b) { return ((uint64_t)b.n_seqs + 1) * 8 + 15 & ~15ull; }
+
 uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b) {
-  (void)c;
-  (void)b;
-  return 16;
+  return kvq8_prefix_bytes(b) + 2ull * kvq8_runs(c, b) * (8 * c.hd + 16) * 4;
 }
 
 template <int HD, typename T>
 static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
-  launch_pdl(k_kvq8_attend<HD, T>, dim3(a.b.max_new, a.c.nkv * a.c.group, a.b.n_seqs), dim3(KQ_AT_THREADS), 0, s, a.c,
-             a.b, static_cast<const T*>(a.q), a.ldq, static_cast<T*>(a.out), a.ldo, a.window, a.sinks, a.scale);
+  const size_t smem = sizeof(KqSplitSmem<HD>);
+  CK(cudaFuncSetAttribute(k_kvq8_split<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const uint32_t runs = kvq8_runs(a.c, a.b);
+  KqSplitArgs<HD, T> k{a.c,
+                       a.b,
+                       static_cast<const T*>(a.q),
+                       static_cast<T*>(a.out),
+                       a.ldq,
+                       a.ldo,
+                       a.window,
+                       a.sinks,
+                       a.scale * 1.44269504088896341f,
+                       static_cast<uint64_t*>(a.work),
+                       reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b))};
+  launch_pdl(k_kvq8_split<HD, T>, dim3(runs), dim3(KQ_SP_THREADS), smem, s, k);
+  launch_pdl(k_kvq8_merge<HD, T>, dim3(a.b.max_new * a.c.group, a.c.nkv, a.b.n_seqs), dim3(KQ_MG_THREADS), 0, s, k,
+             runs);
 }
 
 void launch_kvq8_attend(const KvQ8Attend& a, cudaStream_t s) {
