@@ -194,30 +194,37 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // k_kvq8_merge joins.
 //
 // The cache bytes bound the kernel, so everything else has to fit under them.
-// One warp takes 16 positions (a block) of the page.  Codes become fp16
-// exactly (0x6400 | byte is 1024 + byte: one byte permute and one subtraction
-// for two of them) and both products run on mma.m16n8k16: its 16 rows are the
-// 8 query rows twice, as the high and the low part of an 11 + 11 bit split, so
-// that the products keep f32's precision at no further cost.  The block's
-// scales stay outside: the keys' multiplies the score, the values' the
-// probability before its split.
+// A CTA walks its pages two at a time, a warp taking 32 positions (two blocks)
+// of one.  Codes become fp16 exactly (0x6400 | byte is 1024 + byte: one byte
+// permute and one subtraction for two of them) and both products run on
+// mma.m16n8k16: its 16 rows are the 8 query rows twice, as the high and the low
+// part of an 11 + 11 bit split, so that the products keep f32's precision at no
+// further cost.  The block's scales stay outside: the keys' multiplies the
+// score, the values' the probability before its split.  The tensor cores'
+// additions truncate, which over a long run would shrink the sums (2.6e-6 after
+// 148 of them), so a warp's 32 positions are summed from zero and then added
+// to the running sums in f32.
 //
 // Softmax: with scores x_t (base 2) and value scales v_t the running maximum m
 // is taken over x_t + log2 v_t.  The weights w_t = 2^(x_t - m) v_t that
 // multiply the codes are then at most 1, whatever the scales, and l = sum
-// 2^(x_t - m) is the denominator.  Scales under 2^-100 count as that in m, so
-// that l stays finite.
+// 2^(x_t - m) is the denominator.  m follows that maximum only when it falls
+// behind by 2^8 (fp16 holds the weights up to there), so that the sums are
+// seldom rescaled.  Scales under 2^-100 count as that in m, so that l stays
+// finite.
 // ---------------------------------------------------------------------------
 constexpr int KQ_SP_THREADS = 128;
-constexpr uint32_t KQ_SP_STAGES = 4;     // tiles in flight per warp
+constexpr uint32_t KQ_SP_STAGES = 2;     // tiles of a warp in shared memory
 constexpr uint32_t KQ_SP_CTAS = 3;       // CTAs per SM
+constexpr uint32_t KQ_SP_POS = 32;       // positions of a page that a warp takes
+constexpr float KQ_LAG = 8.f;            // m is at most this far behind (base 2)
 constexpr float KQ_MIN_SCALE = 7.8886090522101181e-31f;  // 2^-100
 
 template <int HD>
 struct KqSplitSmem {
   struct Stage {
-    uint8_t k[KQ_BLOCK * HD], v[KQ_BLOCK * HD];
-    float scale[4];  // keys, values
+    uint8_t k[KQ_SP_POS * HD], v[KQ_SP_POS * HD];
+    float ks[2], vs[2];  // the two blocks' scales
   };
   union {
     Stage ring[KQ_SP_THREADS / 32][KQ_SP_STAGES];
@@ -225,7 +232,7 @@ struct KqSplitSmem {
   };
   __half qh[8][HD], ql[8][HD];
   float rowf[8];
-  int32_t rowpos[8];
+  uint32_t rowpos[8];
   float m[KQ_SP_THREADS / 32][8], l[KQ_SP_THREADS / 32][8];
   uint64_t scan[KQ_SP_THREADS / 32];
 };
@@ -296,8 +303,13 @@ __device__ __forceinline__ void kq_split2(float a, float b, uint32_t* hi, uint32
 __device__ __forceinline__ void kq_cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void kq_cp4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void kq_cp8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ float kq_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Partial results: one slot per run end.  A slot holds the 8 rows' sums of
@@ -322,10 +334,11 @@ struct KqSplitArgs {
 
 // Rows of one segment in shared memory: rotated, scaled by a power of two to
 // a largest magnitude in [2^13, 2^14), split.  rowf undoes the power and holds
-// the softmax scale; rowpos is the row's position, -1 for a row that is none.
+// the softmax scale; rowpos is the row's position (rows that are none are
+// zeros at position phi; nothing of them is written).
 template <int HD, typename T>
 __device__ __forceinline__ void kq_load_rows(const KqSplitArgs<HD, T>& a, KqSplitSmem<HD>& sm, const KqSeq& s,
-                                             uint32_t kvh, uint32_t grp) {
+                                             uint32_t kvh, uint32_t grp, uint32_t phi) {
   constexpr uint32_t half = HD / 2, N = half / 16;  // pairs per thread
   const uint32_t r = threadIdx.x >> 4, l16 = threadIdx.x & 15, rr = grp * 8 + r, j = rr / a.c.group;
   const bool live = j < (uint32_t)s.n_new;
@@ -367,7 +380,7 @@ __device__ __forceinline__ void kq_load_rows(const KqSplitArgs<HD, T>& a, KqSpli
   }
   if (l16 == 0) {
     sm.rowf[r] = a.scale * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-    sm.rowpos[r] = live ? (int32_t)pos : -1;
+    sm.rowpos[r] = live ? pos : phi;
   }
 }
 
@@ -380,10 +393,11 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
   pdl_trigger();
   pdl_wait();
   // this CTA's run of tiles [w0, w1) and the sequence it starts in
-  uint64_t total = 0;
+  uint64_t total = 0, mine = 0;  // mine: the tiles of sequence tid
   for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
     const uint32_t i = i0 + tid;
     uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv) : 0;
+    if (i0 == 0) mine = n;
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     if (lane == 0) sm.scan[warp] = n;
     __syncthreads();
@@ -399,7 +413,9 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
     __shared__ uint64_t s_off;
     for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
       const uint32_t i = i0 + tid;
-      const uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv) : 0;
+      const uint64_t n = i0 == 0              ? mine
+                         : i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv)
+                                          : 0;
       uint64_t inc = n;
       for (int o = 1; o < 32; o <<= 1) {
         const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
@@ -442,41 +458,46 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
     const uint32_t j0 = grp * 8 / a.c.group, j1 = min((grp * 8 + 7) / a.c.group, (uint32_t)p.s.n_new - 1);
     const uint32_t plo = p.s.len - p.s.n_new + j0, phi = p.s.len - p.s.n_new + j1;  // the group's positions
 
-    // pages of the next 32 tiles, one per lane, and of the 32 after them
-    const int32_t last = (int32_t)nv - 1;
-    auto page_of = [&](uint32_t i) { return max(kq_page(a.c, a.b, seq, p.span.page(v0 + min((int32_t)i, last))), 0); };
-    int32_t pid = page_of(lane), pid_next = nv > 32 ? page_of(32 + lane) : 0;
+    // the warp's tiles: pages v0 + 2 i + warp / 2, positions 32 (warp % 2) ..
+    const uint32_t side = warp >> 1, sub = warp & 1;
+    const uint32_t nt = (nv - min(nv, side) + 1) / 2;
+    // pages of the next 32 of them, one per lane, and of the 32 after those
+    auto page_of = [&](uint32_t i) {
+      return max(kq_page(a.c, a.b, seq, p.span.page(v0 + min(2 * i + side, nv - 1))), 0);
+    };
+    int32_t pid = page_of(lane), pid_next = nt > 32 ? page_of(32 + lane) : 0;
     uint32_t issued = 0;
-    // the warp's block of tile i, unless none of the group's rows sees it
-    auto block_pos = [&](uint32_t i) { return p.span.page(v0 + i) * KQ_PAGE + warp * KQ_BLOCK; };
+    auto tile_pos = [&](uint32_t i) { return p.span.page(v0 + 2 * i + side) * KQ_PAGE + sub * KQ_SP_POS; };
+    // whether none of the group's rows sees any of the tile
     auto dead = [&](uint32_t pos) {
-      return pos > phi || (a.window && pos + KQ_BLOCK <= plo && plo - (pos + KQ_BLOCK - 1) >= a.window && pos >= a.sinks);
+      return pos > phi ||
+             (a.window && pos + KQ_SP_POS <= plo && plo - (pos + KQ_SP_POS - 1) >= a.window && pos >= a.sinks);
     };
     auto issue = [&]() {
       const uint32_t i = issued++;
-      if (i < nv) {
+      if (i < nt) {
         if (i && i % 32 == 0) {
           pid = pid_next;
-          pid_next = i + 32 < nv ? page_of(i + 32 + lane) : 0;
+          pid_next = i + 32 < nt ? page_of(i + 32 + lane) : 0;
         }
         const int32_t page = __shfl_sync(0xffffffffu, pid, i % 32);
-        if (!dead(block_pos(i))) {
+        if (!dead(tile_pos(i))) {
           auto& st = sm.ring[warp][i % KQ_SP_STAGES];
-          const uint64_t side = ((uint64_t)page * a.c.nkv + kvh) * 2;
-          const uint8_t* src = a.c.codes + side * KQ_PAGE * HD + warp * KQ_BLOCK * HD;
+          const uint64_t at = ((uint64_t)page * a.c.nkv + kvh) * 2;
+          const uint8_t* src = a.c.codes + at * KQ_PAGE * HD + sub * KQ_SP_POS * HD + lane * 16;
 #pragma unroll
-          for (uint32_t x = 0; x < KQ_BLOCK * HD / 512; x++) {
-            kq_cp16(st.k + x * 512 + lane * 16, src + x * 512 + lane * 16);
-            kq_cp16(st.v + x * 512 + lane * 16, src + KQ_PAGE * HD + x * 512 + lane * 16);
+          for (uint32_t x = 0; x < KQ_SP_POS * HD / 512; x++) {
+            kq_cp16(st.k + x * 512 + lane * 16, src + x * 512);
+            kq_cp16(st.v + x * 512 + lane * 16, src + KQ_PAGE * HD + x * 512);
           }
-          if (lane < 2) kq_cp4(&st.scale[lane], a.c.scales + (side + lane) * KQ_NB + warp);
+          if (lane < 2) kq_cp8(lane ? st.vs : st.ks, a.c.scales + (at + lane) * KQ_NB + sub * 2);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     for (uint32_t i = 0; i + 1 < KQ_SP_STAGES; i++) issue();
 
-    kq_load_rows<HD, T>(a, sm, p.s, kvh, grp);
+    kq_load_rows<HD, T>(a, sm, p.s, kvh, grp, phi);
     __syncthreads();
     uint32_t qh[KJ][8], ql[KJ][8];  // row g, dims 64j + 16t .. + 15
 #pragma unroll
@@ -487,81 +508,95 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
         ql[j][i] = *reinterpret_cast<const uint32_t*>(&sm.ql[g][j * 64 + t * 16 + 2 * i]);
       }
     const float rowf = sm.rowf[g];
-    const int32_t rowpos = sm.rowpos[g];
-    float m = -INFINITY, l = 0.f, o[HD / 8][4];
+    const uint32_t rowpos = sm.rowpos[g];
+    float m = -INFINITY, l = 0.f, o[HD / 8][2];
 #pragma unroll
-    for (int n = 0; n < HD / 8; n++)
-#pragma unroll
-      for (int x = 0; x < 4; x++) o[n][x] = 0.f;
+    for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = 0.f;
 
-    for (uint32_t i = 0; i < nv; i++) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(KQ_SP_STAGES - 2) : "memory");
-      __syncwarp();  // every lane's copies have landed, and every lane is done with the stage refilled next
+    for (uint32_t i = 0; i < nt; i++) {
+      __syncwarp();  // every lane is done with the stage refilled next
       issue();
-      const uint32_t pos = block_pos(i);
+      asm volatile("cp.async.wait_group %0;" ::"n"(KQ_SP_STAGES - 1) : "memory");
+      __syncwarp();  // every lane's copies of tile i have landed
+      const uint32_t pos = tile_pos(i);
       if (dead(pos)) continue;
       auto& st = sm.ring[warp][i % KQ_SP_STAGES];
-      float sacc[2][4] = {};
+      float x[8];  // scores: block k / 4, positions 8 (k / 2 % 2) + 2t + k % 2 of it
 #pragma unroll
-      for (uint32_t n = 0; n < 2; n++)
+      for (uint32_t n = 0; n < 4; n++) {
+        float acc[4] = {};
 #pragma unroll
         for (uint32_t j = 0; j < KJ; j++) {
           const uint4 kw = *reinterpret_cast<const uint4*>(st.k + n * 8 * HD + j * 512 + lane * 16);
           const uint32_t word[4] = {kw.x, kw.y, kw.z, kw.w};
 #pragma unroll
-          for (uint32_t x = 0; x < 4; x++) {
+          for (uint32_t y = 0; y < 4; y++) {
             uint32_t h[2];
-            kq_halves(word[x], h);
-            const uint32_t qa[4] = {qh[j][2 * x], ql[j][2 * x], qh[j][2 * x + 1], ql[j][2 * x + 1]};
-            kq_mma(sacc[n], qa, h[0], h[1]);
+            kq_halves(word[y], h);
+            const uint32_t qa[4] = {qh[j][2 * y], ql[j][2 * y], qh[j][2 * y + 1], ql[j][2 * y + 1]};
+            kq_mma(acc, qa, h[0], h[1]);
           }
         }
-      const float ks = st.scale[0] * rowf, vs = st.scale[1];
-      float x[4];
+        const float f = st.ks[n >> 1] * rowf;
+        x[2 * n] = fmaf(acc[2], 1.f / 2048.f, acc[0]) * f;
+        x[2 * n + 1] = fmaf(acc[3], 1.f / 2048.f, acc[1]) * f;
+      }
+      uint32_t hidden = 0;
+      if (pos + KQ_SP_POS - 1 > plo ||
+          (a.window && pos + KQ_SP_POS > a.sinks && phi - pos >= a.window)) {  // some row does not see all of it
 #pragma unroll
-      for (int k = 0; k < 4; k++) x[k] = fmaf(sacc[k >> 1][2 + (k & 1)], 1.f / 2048.f, sacc[k >> 1][k & 1]) * ks;
-      if (!(pos + KQ_BLOCK - 1 <= plo &&
-            (!a.window || pos + KQ_BLOCK - 1 < a.sinks || pos > phi || phi - pos < a.window) && rowpos >= 0)) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int32_t at = (int32_t)pos + (k >> 1) * 8 + 2 * t + (k & 1);
-          const bool seen =
-              at <= rowpos && (!a.window || (uint32_t)(rowpos - at) < a.window || (uint32_t)at < a.sinks);
-          if (!seen) x[k] = -INFINITY;
+        for (int k = 0; k < 8; k++) {
+          const uint32_t at = pos + (k >> 1) * 8 + 2 * t + (k & 1);
+          const bool seen = at <= rowpos && (!a.window || rowpos - at < a.window || at < a.sinks);
+          if (!seen) {
+            x[k] = -INFINITY;
+            hidden |= 1u << k;
+          }
         }
       }
-      float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) + __log2f(fmaxf(vs, KQ_MIN_SCALE));
+      const float va = st.vs[0], vb = st.vs[1];
+      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) + __log2f(fmaxf(va, KQ_MIN_SCALE)),
+                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) + __log2f(fmaxf(vb, KQ_MIN_SCALE)));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(m, top), sub = mn == -INFINITY ? 0.f : mn;
-      const float alpha = mn == m ? 1.f : exp2f(m - sub);
-      m = mn;
-      float wv[4], ps = 0.f;
+      if (__any_sync(0xffffffffu, top > m + KQ_LAG)) {
+        const float mn = fmaxf(m, top), f = mn == m ? 1.f : kq_exp2(m - mn);
+        m = mn;
+        l *= f;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float e = exp2f(x[k] - sub);
-        ps += e;
-        wv[k] = x[k] == -INFINITY ? 0.f : e * vs;
+        for (int n = 0; n < HD / 8; n++) o[n][0] *= f, o[n][1] *= f;
       }
-      l = fmaf(l, alpha, ps);
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+      const float sub_m = m == -INFINITY ? 0.f : m;
+      float wv[8];
 #pragma unroll
-        for (int n = 0; n < HD / 8; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) o[n][k] *= alpha;
+      for (int k = 0; k < 8; k++) {
+        const float e = kq_exp2(x[k] - sub_m);
+        l += e;
+        wv[k] = e * (k < 4 ? va : vb);
       }
-      uint32_t pa[4];
-      kq_split2(wv[0], wv[1], &pa[0], &pa[1]);
-      kq_split2(wv[2], wv[3], &pa[2], &pa[3]);
+      if (hidden) {  // 0, whatever the scale of a block without positions of the sequence
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (hidden >> k & 1) wv[k] = 0.f;
+      }
+      uint32_t pa[2][4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) kq_split2(wv[2 * k], wv[2 * k + 1], &pa[k >> 1][2 * (k & 1)], &pa[k >> 1][2 * (k & 1) + 1]);
 #pragma unroll
       for (uint32_t n = 0; n < NQ; n++) {
-        const uint4 vw = *reinterpret_cast<const uint4*>(st.v + n * 512 + lane * 16);
-        const uint32_t word[4] = {vw.x, vw.y, vw.z, vw.w};
+        const uint4 wa = *reinterpret_cast<const uint4*>(st.v + n * 512 + lane * 16);
+        const uint4 wb = *reinterpret_cast<const uint4*>(st.v + KQ_BLOCK * HD + n * 512 + lane * 16);
+        const uint32_t word[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
+          float d[4] = {};
           uint32_t h[2];
           kq_halves(word[k], h);
-          kq_mma(o[n * 4 + k], pa, h[0], h[1]);
+          kq_mma(d, pa[0], h[0], h[1]);
+          kq_halves(word[4 + k], h);
+          kq_mma(d, pa[1], h[0], h[1]);
+          o[n * 4 + k][0] += fmaf(d[2], 1.f / 2048.f, d[0]);
+          o[n * 4 + k][1] += fmaf(d[3], 1.f / 2048.f, d[1]);
         }
       }
     }
@@ -575,8 +610,7 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
     }
 #pragma unroll
     for (int n = 0; n < HD / 8; n++)
-      *reinterpret_cast<float2*>(&sm.acc[warp][g][n * 8 + 2 * t]) =
-          make_float2(fmaf(o[n][2], 1.f / 2048.f, o[n][0]), fmaf(o[n][3], 1.f / 2048.f, o[n][1]));
+      *reinterpret_cast<float2*>(&sm.acc[warp][g][n * 8 + 2 * t]) = make_float2(o[n][0], o[n][1]);
     __syncthreads();
     const bool whole = nv == p.span.n;
     // a run has at most two pieces that are not whole segments: its first and its last
@@ -704,6 +738,18 @@ void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, v
     f16 ? kvq8_read_t<64, __half>(c, b, k, v, ld, s) : kvq8_read_t<64, float>(c, b, k, v, ld, s);
 }
 
+// Runs f once for each device (a kernel's attributes hold per device); devices
+// past the 64 bits run it every time.
+template <class F>
+static void kvq8_once(std::atomic<uint64_t>& ready, F&& f) {
+  int dev = 0;
+  CK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (ready.load(std::memory_order_acquire) & bit) return;
+  f();
+  ready.fetch_or(bit, std::memory_order_release);
+}
+
 // Runs of the split form: every SM filled, never more than there can be tiles.
 static uint32_t kvq8_runs(const KvQ8Dev& c, const KvQ8Batch& b) {
   const uint64_t most = (uint64_t)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8) * b.max_pages;
@@ -718,7 +764,10 @@ uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b) {
 template <int HD, typename T>
 static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
   const size_t smem = sizeof(KqSplitSmem<HD>);
-  CK(cudaFuncSetAttribute(k_kvq8_split<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> ready{0};
+  kvq8_once(ready, [&] {
+    CK(cudaFuncSetAttribute(k_kvq8_split<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  });
   const uint32_t runs = kvq8_runs(a.c, a.b);
   KqSplitArgs<HD, T> k{a.c,
                        a.b,
