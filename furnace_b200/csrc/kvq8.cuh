@@ -186,12 +186,15 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // ---------------------------------------------------------------------------
 // Attention of few rows over long caches (k_kvq8_split + k_kvq8_merge).
 //
-// A tile is one page of one KV head for one group of 8 rows (row = (new token,
-// query head of the KV head)).  All tiles of the call, sequence by sequence,
-// are cut into equal runs, one per CTA, so that ragged batches load the SMs
-// evenly; a run may hold several segments ((sequence, KV head, row group)) and
-// a segment may span several runs: it is then written as partial results that
-// k_kvq8_merge joins.
+// A segment is one KV head of one sequence for one group of 8 rows (row = (new
+// token, query head of the KV head)).  It costs its pages plus KQ_SEG: loading
+// the rows and writing the result take about as long.  All segments of the
+// call, sequence by sequence, are cut into equal runs of that cost, one per
+// CTA, so that ragged batches load the SMs evenly; a run may hold several
+// segments, and a segment may span several runs: it is then written as partial
+// results that k_kvq8_merge joins.  Where no sequence has more than
+// KQ_WHOLE_PAGES pages every segment is a CTA of its own (k_kvq8_whole):
+// nothing to plan and nothing to join.
 //
 // The cache bytes bound the kernel, so everything else has to fit under them.
 // A CTA walks its pages two at a time, a warp taking 32 positions (two blocks)
@@ -218,6 +221,8 @@ constexpr uint32_t KQ_SP_STAGES = 2;     // tiles of a warp in shared memory
 constexpr uint32_t KQ_SP_CTAS = 3;       // CTAs per SM
 constexpr uint32_t KQ_SP_POS = 32;       // positions of a page that a warp takes
 constexpr float KQ_LAG = 8.f;            // m is at most this far behind (base 2)
+constexpr uint32_t KQ_SEG = 2;           // a segment's cost besides its pages, in pages
+constexpr uint32_t KQ_WHOLE_PAGES = 4;
 constexpr float KQ_MIN_SCALE = 7.8886090522101181e-31f;  // 2^-100
 
 template <int HD>
@@ -228,7 +233,7 @@ struct KqSplitSmem {
   };
   union {
     Stage ring[KQ_SP_THREADS / 32][KQ_SP_STAGES];
-    float acc[KQ_SP_THREADS / 32][8][HD];  // the warps' sums at a segment's end
+    float acc[KQ_SP_THREADS / 32][8][HD + 8];  // the warps' sums at a segment's end
   };
   __half qh[8][HD], ql[8][HD];
   float rowf[8];
@@ -258,7 +263,7 @@ struct KqPlan {
   KqSeq s;
   KqSpan span;
   uint32_t groups;  // row groups of one KV head
-  __device__ __forceinline__ uint64_t tiles(uint32_t nkv) const { return (uint64_t)groups * span.n * nkv; }
+  __device__ __forceinline__ uint64_t cost(uint32_t nkv) const { return (uint64_t)groups * (span.n + KQ_SEG) * nkv; }
 };
 __device__ __forceinline__ KqPlan kq_plan(const KvQ8Dev& c, const KvQ8Batch& b, uint32_t i, uint32_t window,
                                           uint32_t sinks) {
@@ -312,6 +317,11 @@ __device__ __forceinline__ float kq_exp2(float x) {
   return y;
 }
 
+// Length of a run: even, so that a run's pages come in pairs.
+__device__ __forceinline__ uint64_t kq_per(uint64_t total, uint32_t runs) {
+  return (total + 2ull * runs - 1) / (2ull * runs) * 2;
+}
+
 // Partial results: one slot per run end.  A slot holds the 8 rows' sums of
 // codes, then their m, then their l.
 template <int HD>
@@ -328,135 +338,116 @@ struct KqSplitArgs {
   uint64_t ldq, ldo;
   uint32_t window, sinks;
   float scale;          // softmax scale * log2(e)
-  uint64_t* prefix;     // [n_seqs + 1] tiles before each sequence (written by CTA 0)
+  uint64_t* prefix;     // [n_seqs + 1] cost before each sequence (written by CTA 0)
   float* slots;         // [2 * gridDim.x]
 };
 
-// Rows of one segment in shared memory: rotated, scaled by a power of two to
-// a largest magnitude in [2^13, 2^14), split.  rowf undoes the power and holds
-// the softmax scale; rowpos is the row's position (rows that are none are
-// zeros at position phi; nothing of them is written).
-template <int HD, typename T>
-__device__ __forceinline__ void kq_load_rows(const KqSplitArgs<HD, T>& a, KqSplitSmem<HD>& sm, const KqSeq& s,
-                                             uint32_t kvh, uint32_t grp, uint32_t phi) {
-  constexpr uint32_t half = HD / 2, N = half / 16;  // pairs per thread
-  const uint32_t r = threadIdx.x >> 4, l16 = threadIdx.x & 15, rr = grp * 8 + r, j = rr / a.c.group;
-  const bool live = j < (uint32_t)s.n_new;
-  const uint32_t pos = s.len - s.n_new + j;
-  float x[2 * N], top = 0.f;
-#pragma unroll
-  for (uint32_t i = 0; i < N; i++) {
-    const uint32_t d = l16 * N + i;
-    float u = 0.f, w = 0.f;
-    if (live) {
-      const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d;
-      u = kq_ld(p);
-      w = kq_ld(p + half);
-      if (a.c.rope) {
-        const float2 f = a.c.rope[(uint64_t)pos * half + d];
-        const float v = __fsub_rn(__fmul_rn(u, f.x), __fmul_rn(w, f.y));
-        w = __fadd_rn(__fmul_rn(u, f.y), __fmul_rn(w, f.x));
-        u = v;
-      }
-    }
-    x[i] = u;
-    x[N + i] = w;
-    top = fmaxf(top, fmaxf(fabsf(u), fabsf(w)));
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-  e = max(e, -100);
-  const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);  // e <= 128: the exponent stays positive
-#pragma unroll
-  for (uint32_t i = 0; i < N; i++) {
-#pragma unroll
-    for (uint32_t k = 0; k < 2; k++) {
-      const float v = x[k * N + i] * up;
-      const __half hi = __float2half_rn(v);
-      sm.qh[r][k * half + l16 * N + i] = hi;
-      sm.ql[r][k * half + l16 * N + i] = __float2half_rn((v - __half2float(hi)) * 2048.f);
-    }
-  }
-  if (l16 == 0) {
-    sm.rowf[r] = a.scale * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-    sm.rowpos[r] = live ? pos : phi;
+// A row's elements d .. d + N - 1 (N consecutive, aligned).
+template <int N>
+__device__ __forceinline__ void kq_ldn(const float* p, float* x) {
+  if constexpr (N == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x, x[1] = v.y;
   }
 }
-
-template <int HD, typename T>
-__global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const __grid_constant__ KqSplitArgs<HD, T> a) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
-  constexpr uint32_t KJ = HD / 64, NQ = HD / 32;
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  pdl_trigger();
-  pdl_wait();
-  // this CTA's run of tiles [w0, w1) and the sequence it starts in
-  uint64_t total = 0, mine = 0;  // mine: the tiles of sequence tid
-  for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
-    const uint32_t i = i0 + tid;
-    uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv) : 0;
-    if (i0 == 0) mine = n;
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (lane == 0) sm.scan[warp] = n;
-    __syncthreads();
-    for (int w = 0; w < KQ_SP_THREADS / 32; w++) total += sm.scan[w];
-    __syncthreads();
-  }
-  const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
-  const uint64_t w0 = min(per * blockIdx.x, total), w1 = min(w0 + per, total);
-  uint64_t before = 0, off = 0;
-  uint32_t seq = 0;
-  if (a.b.n_seqs > 1 || blockIdx.x == 0) {
-    __shared__ uint32_t s_seq;
-    __shared__ uint64_t s_off;
-    for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
-      const uint32_t i = i0 + tid;
-      const uint64_t n = i0 == 0              ? mine
-                         : i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).tiles(a.c.nkv)
-                                          : 0;
-      uint64_t inc = n;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= (uint32_t)o) inc += x;
-      }
-      if (lane == 31) sm.scan[warp] = inc;
-      __syncthreads();
-      uint64_t base = before;
-      for (uint32_t w = 0; w < KQ_SP_THREADS / 32; w++) {
-        if (w < warp) base += sm.scan[w];
-        before += sm.scan[w];
-      }
-      if (blockIdx.x == 0 && i < a.b.n_seqs) a.prefix[i] = base + inc - n;
-      if (n && w0 >= base + inc - n && w0 < base + inc) {
-        s_seq = i;
-        s_off = w0 - (base + inc - n);
-      }
-      __syncthreads();
-    }
-    if (blockIdx.x == 0 && tid == 0) a.prefix[a.b.n_seqs] = total;
-    if (w0 < w1) {
-      seq = s_seq;
-      off = s_off;
-    }
+template <int N>
+__device__ __forceinline__ void kq_ldn(const __half* p, float* x) {
+  uint32_t w[N / 2];
+  if constexpr (N == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
   } else {
-    off = w0;
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-  if (w0 >= w1) return;
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void kq_st4(float* p, const float* x) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void kq_st4(__half* p, const float* x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(kq_pack(x[0], x[1]), kq_pack(x[2], x[3]));
+}
 
-  KqPlan p = kq_plan(a.c, a.b, seq, a.window, a.sinks);
-  uint64_t w = w0;
-  while (w < w1) {
-    while (off >= p.tiles(a.c.nkv)) {
-      off -= p.tiles(a.c.nkv);
-      p = kq_plan(a.c, a.b, ++seq, a.window, a.sinks);  // w < total: a later sequence has tiles
+// Rows of one segment: 16 threads a row, each N pairs.  get() starts the
+// loads; put() rotates, scales the row by a power of two to a largest
+// magnitude in [2^13, 2^14) and leaves its two parts in shared memory.  rowf
+// undoes the power and holds the softmax scale; rowpos is the row's position
+// (rows that are none are zeros at position phi; nothing of them is written).
+template <int HD, typename T>
+struct KqRows {
+  static constexpr uint32_t half = HD / 2, N = half / 16;
+  float x[2 * N], f[2 * N];
+  bool live;
+  uint32_t pos;
+  __device__ __forceinline__ void get(const KqSplitArgs<HD, T>& a, const KqSeq& s, uint32_t kvh, uint32_t grp) {
+    const uint32_t rr = grp * 8 + (threadIdx.x >> 4), j = rr / a.c.group, d = (threadIdx.x & 15) * N;
+    live = j < (uint32_t)s.n_new;
+    pos = s.len - s.n_new + j;
+#pragma unroll
+    for (uint32_t i = 0; i < 2 * N; i++) x[i] = 0.f, f[i] = i % 2 ? 0.f : 1.f;
+    if (live) {
+      const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d;
+      kq_ldn<N>(p, x);
+      kq_ldn<N>(p + half, x + N);
+      if (a.c.rope) {
+        const float* r = reinterpret_cast<const float*>(a.c.rope + (uint64_t)pos * half + d);
+        kq_ldn<N>(r, f);
+        kq_ldn<N>(r + N, f + N);
+      }
     }
-    const uint32_t seg = (uint32_t)(off / p.span.n), v0 = (uint32_t)(off % p.span.n);
-    const uint32_t nv = (uint32_t)min((uint64_t)(p.span.n - v0), w1 - w);
-    const uint32_t kvh = seg / p.groups, grp = seg % p.groups;
+  }
+  __device__ __forceinline__ void put(const KqSplitArgs<HD, T>& a, KqSplitSmem<HD>& sm, uint32_t phi) {
+    const uint32_t r = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    float top = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+      const float u = x[i], w = x[N + i];
+      if (a.c.rope) {
+        x[i] = __fsub_rn(__fmul_rn(u, f[2 * i]), __fmul_rn(w, f[2 * i + 1]));
+        x[N + i] = __fadd_rn(__fmul_rn(u, f[2 * i + 1]), __fmul_rn(w, f[2 * i]));
+      }
+      top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(x[N + i])));
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+    e = max(e, -100);
+    const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);  // e <= 128: the exponent stays positive
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++)
+#pragma unroll
+      for (uint32_t i = 0; i < N; i += 2) {
+        uint32_t hi, lo;
+        kq_split2(x[k * N + i] * up, x[k * N + i + 1] * up, &hi, &lo);
+        *reinterpret_cast<uint32_t*>(&sm.qh[r][k * half + l16 * N + i]) = hi;
+        *reinterpret_cast<uint32_t*>(&sm.ql[r][k * half + l16 * N + i]) = lo;
+      }
+    if (l16 == 0) {
+      sm.rowf[r] = a.scale * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+      sm.rowpos[r] = live ? pos : phi;
+    }
+  }
+};
+
+// Pages v0 .. v0 + nv - 1 of a segment.  The result goes to out where these
+// are all of its pages, else to the slot.  Called by the whole CTA.
+template <int HD, typename T>
+__device__ __forceinline__ void kq_segment(const KqSplitArgs<HD, T>& a, KqSplitSmem<HD>& sm, const KqPlan& p,
+                                           uint32_t seq, uint32_t kvh, uint32_t grp, uint32_t v0, uint32_t nv,
+                                           float* slot) {
+    constexpr uint32_t KJ = HD / 64, NQ = HD / 32;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t j0 = grp * 8 / a.c.group, j1 = min((grp * 8 + 7) / a.c.group, (uint32_t)p.s.n_new - 1);
     const uint32_t plo = p.s.len - p.s.n_new + j0, phi = p.s.len - p.s.n_new + j1;  // the group's positions
+    KqRows<HD, T> rows;
+    rows.get(a, p.s, kvh, grp);
 
     // the warp's tiles: pages v0 + 2 i + warp / 2, positions 32 (warp % 2) ..
     const uint32_t side = warp >> 1, sub = warp & 1;
@@ -497,7 +488,7 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
     };
     for (uint32_t i = 0; i + 1 < KQ_SP_STAGES; i++) issue();
 
-    kq_load_rows<HD, T>(a, sm, p.s, kvh, grp, phi);
+    rows.put(a, sm, phi);
     __syncthreads();
     uint32_t qh[KJ][8], ql[KJ][8];  // row g, dims 64j + 16t .. + 15
 #pragma unroll
@@ -613,35 +604,130 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
       *reinterpret_cast<float2*>(&sm.acc[warp][g][n * 8 + 2 * t]) = make_float2(o[n][0], o[n][1]);
     __syncthreads();
     const bool whole = nv == p.span.n;
-    // a run has at most two pieces that are not whole segments: its first and its last
-    float* slot = a.slots + (2ull * blockIdx.x + (w != w0)) * kq_slot_floats<HD>();
-    for (uint32_t x = tid; x < 8 * HD; x += KQ_SP_THREADS) {
-      const uint32_t r = x / HD, d = x % HD;
+    // a row is HD / 4 lanes, four dims each
+    constexpr uint32_t L = HD / 4, RPP = KQ_SP_THREADS / L;  // lanes per row, rows per pass
+#pragma unroll
+    for (uint32_t r0 = 0; r0 < 8; r0 += RPP) {
+      const uint32_t r = r0 + tid / L, d = tid % L * 4;
       const float top = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
-      float num = 0.f, den = 0.f;
+      float num[4] = {}, den = 0.f;
 #pragma unroll
       for (int y = 0; y < KQ_SP_THREADS / 32; y++) {
-        const float f = sm.m[y][r] == -INFINITY ? 0.f : exp2f(sm.m[y][r] - top);
-        num = fmaf(f, sm.acc[y][r][d], num);
+        const float f = sm.m[y][r] == -INFINITY ? 0.f : kq_exp2(sm.m[y][r] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&sm.acc[y][r][d]);
+        num[0] = fmaf(f, v.x, num[0]);
+        num[1] = fmaf(f, v.y, num[1]);
+        num[2] = fmaf(f, v.z, num[2]);
+        num[3] = fmaf(f, v.w, num[3]);
         den = fmaf(f, sm.l[y][r], den);
       }
       if (whole) {
         const uint32_t rr = grp * 8 + r, j = rr / a.c.group;
-        if (j < (uint32_t)p.s.n_new)
-          kq_st(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d,
-                den == 0.f ? 0.f : __fdiv_rn(num, den));
+        if (j < (uint32_t)p.s.n_new) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) num[i] = den == 0.f ? 0.f : __fdiv_rn(num[i], den);
+          kq_st4(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d, num);
+        }
       } else {
-        slot[x] = num;
+        kq_st4(slot + r * HD + d, num);
         if (d == 0) {
           slot[8 * HD + r] = top;
           slot[8 * HD + 8 + r] = den;
         }
       }
     }
-    __syncthreads();  // shared memory is reused by the next segment
-    w += nv;
-    off += nv;
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const __grid_constant__ KqSplitArgs<HD, T> a) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_trigger();  // after the wait: what the merge reads of the inputs is final when it starts
+  // this CTA's run [w0, w1) of the call's cost and the sequence it starts in
+  uint64_t total = 0, mine = 0;  // mine: the cost of sequence tid
+  for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
+    const uint32_t i = i0 + tid;
+    uint64_t n = i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).cost(a.c.nkv) : 0;
+    if (i0 == 0) mine = n;
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) sm.scan[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < KQ_SP_THREADS / 32; w++) total += sm.scan[w];
+    __syncthreads();
   }
+  const uint64_t per = kq_per(total, gridDim.x);
+  const uint64_t w0 = min(per * blockIdx.x, total), w1 = min(w0 + per, total);
+  uint64_t before = 0, off = 0;
+  uint32_t seq = 0;
+  if (a.b.n_seqs > 1 || blockIdx.x == 0) {
+    __shared__ uint32_t s_seq;
+    __shared__ uint64_t s_off;
+    for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += KQ_SP_THREADS) {
+      const uint32_t i = i0 + tid;
+      const uint64_t n = i0 == 0              ? mine
+                         : i < a.b.n_seqs ? kq_plan(a.c, a.b, i, a.window, a.sinks).cost(a.c.nkv)
+                                          : 0;
+      uint64_t inc = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += x;
+      }
+      if (lane == 31) sm.scan[warp] = inc;
+      __syncthreads();
+      uint64_t base = before;
+      for (uint32_t w = 0; w < KQ_SP_THREADS / 32; w++) {
+        if (w < warp) base += sm.scan[w];
+        before += sm.scan[w];
+      }
+      if (blockIdx.x == 0 && i < a.b.n_seqs) a.prefix[i] = base + inc - n;
+      if (n && w0 >= base + inc - n && w0 < base + inc) {
+        s_seq = i;
+        s_off = w0 - (base + inc - n);
+      }
+      __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) a.prefix[a.b.n_seqs] = total;
+    if (w0 < w1) {
+      seq = s_seq;
+      off = s_off;
+    }
+  } else {
+    off = w0;
+  }
+  if (w0 >= w1) return;
+
+  KqPlan p = kq_plan(a.c, a.b, seq, a.window, a.sinks);
+  for (uint64_t w = w0; w < w1;) {
+    while (off >= p.cost(a.c.nkv)) {
+      off -= p.cost(a.c.nkv);
+      p = kq_plan(a.c, a.b, ++seq, a.window, a.sinks);  // w < total: a later sequence has segments
+    }
+    const uint32_t len = p.span.n + KQ_SEG, seg = (uint32_t)(off / len), u0 = (uint32_t)(off % len);
+    const uint32_t u1 = (uint32_t)min((uint64_t)len, u0 + (w1 - w));
+    const uint32_t v0 = max(u0, KQ_SEG) - KQ_SEG, v1 = max(u1, KQ_SEG) - KQ_SEG;
+    if (v1 > v0) {
+      // a run has at most two pieces that are not whole segments: its first and its last
+      kq_segment<HD, T>(a, sm, p, seq, seg / p.groups, seg % p.groups, v0, v1 - v0,
+                        a.slots + (2ull * blockIdx.x + (w != w0)) * kq_slot_floats<HD>());
+      __syncthreads();  // shared memory is reused by the next segment
+    }
+    w += u1 - u0;
+    off += u1 - u0;
+  }
+}
+
+// Every segment a CTA: grid (nkv * most row groups, n_seqs).
+template <int HD, typename T>
+__global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_whole(const __grid_constant__ KqSplitArgs<HD, T> a) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
+  pdl_wait();
+  pdl_trigger();
+  const KqPlan p = kq_plan(a.c, a.b, blockIdx.y, a.window, a.sinks);
+  const uint32_t kvh = blockIdx.x % a.c.nkv, grp = blockIdx.x / a.c.nkv;
+  if (grp < p.groups) kq_segment<HD, T>(a, sm, p, blockIdx.y, kvh, grp, 0, p.span.n, nullptr);
 }
 
 // Join the pieces of a segment that spans several runs.  Grid (rows of a KV
@@ -652,13 +738,14 @@ constexpr uint32_t KQ_MG_PIECES = 1024;  // runs of a call at most
 template <int HD, typename T>
 __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_constant__ KqSplitArgs<HD, T> a,
                                                               uint32_t runs) {
-  pdl_wait();
-  const KqPlan p = kq_plan(a.c, a.b, blockIdx.z, a.window, a.sinks);
+  const KqPlan p = kq_plan(a.c, a.b, blockIdx.z, a.window, a.sinks);  // inputs: final (see k_kvq8_split)
   const uint32_t rr = blockIdx.x, kvh = blockIdx.y, grp = rr / 8, r = rr % 8, j = rr / a.c.group;
+  pdl_wait();
   if (j >= (uint32_t)p.s.n_new) return;
-  const uint64_t total = a.prefix[a.b.n_seqs], per = (total + runs - 1) / runs;
-  const uint64_t s0 = a.prefix[blockIdx.z] + (uint64_t)(kvh * p.groups + grp) * p.span.n, s1 = s0 + p.span.n;
-  const uint32_t i0 = (uint32_t)(s0 / per), n = (uint32_t)((s1 - 1) / per) - i0 + 1;
+  const uint64_t per = kq_per(a.prefix[a.b.n_seqs], runs);
+  const uint64_t s0 = a.prefix[blockIdx.z] + (uint64_t)(kvh * p.groups + grp) * (p.span.n + KQ_SEG);
+  const uint64_t s1 = s0 + p.span.n + KQ_SEG;
+  const uint32_t i0 = (uint32_t)((s0 + KQ_SEG) / per), n = (uint32_t)((s1 - 1) / per) - i0 + 1;
   if (n == 1) return;  // written by the run itself
   __shared__ float wt[KQ_MG_PIECES];
   __shared__ float red[KQ_MG_THREADS / 32][HD], rden[KQ_MG_THREADS / 32], rtop[KQ_MG_THREADS / 32];
@@ -678,7 +765,7 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
   top = fmaxf(fmaxf(rtop[0], rtop[1]), fmaxf(rtop[2], rtop[3]));
   float den = 0.f;
   for (uint32_t i = tid; i < n; i += KQ_MG_THREADS) {
-    const float f = wt[i] == -INFINITY ? 0.f : exp2f(wt[i] - top);
+    const float f = wt[i] == -INFINITY ? 0.f : kq_exp2(wt[i] - top);
     wt[i] = f;
     den = fmaf(f, slot(i)[8 * HD + 8 + r], den);
   }
@@ -687,7 +774,7 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
   __syncthreads();
   constexpr int DPL = HD / 32;
   float acc[DPL] = {};
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t i = warp; i < n; i += KQ_MG_THREADS / 32) {
     const float* x = slot(i) + r * HD + lane * DPL;
 #pragma unroll
@@ -752,7 +839,7 @@ static void kvq8_once(std::atomic<uint64_t>& ready, F&& f) {
 
 // Runs of the split form: every SM filled, never more than there can be tiles.
 static uint32_t kvq8_runs(const KvQ8Dev& c, const KvQ8Batch& b) {
-  const uint64_t most = (uint64_t)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8) * b.max_pages;
+  const uint64_t most = (uint64_t)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8) * (b.max_pages + KQ_SEG);
   return (uint32_t)std::min<uint64_t>({most, (uint64_t)num_sms() * KQ_SP_CTAS, KQ_MG_PIECES});
 }
 static uint64_t kvq8_prefix_bytes(const KvQ8Batch& b) { return ((uint64_t)b.n_seqs + 1) * 8 + 15 & ~15ull; }
@@ -767,6 +854,7 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
   kvq8_once(ready, [&] {
     CK(cudaFuncSetAttribute(k_kvq8_split<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CK(cudaFuncSetAttribute(k_kvq8_whole<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   });
   const uint32_t runs = kvq8_runs(a.c, a.b);
   KqSplitArgs<HD, T> k{a.c,
@@ -780,6 +868,11 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
                        a.scale * 1.44269504088896341f,
                        static_cast<uint64_t*>(a.work),
                        reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b))};
+  if (a.b.max_pages <= KQ_WHOLE_PAGES) {
+    const uint64_t groups = ((uint64_t)a.b.max_new * a.c.group + 7) / 8;
+    launch_pdl(k_kvq8_whole<HD, T>, dim3((unsigned)(a.c.nkv * groups), a.b.n_seqs), dim3(KQ_SP_THREADS), smem, s, k);
+    return;
+  }
   launch_pdl(k_kvq8_split<HD, T>, dim3(runs), dim3(KQ_SP_THREADS), smem, s, k);
   launch_pdl(k_kvq8_merge<HD, T>, dim3(a.b.max_new * a.c.group, a.c.nkv, a.b.n_seqs), dim3(KQ_MG_THREADS), 0, s, k,
              runs);
