@@ -179,7 +179,7 @@ struct KvQ8Dev {
   uint32_t* status;    // KQ_* bits, set by the kernels
   uint32_t n_pages, n_rope, nkv, group, hd;
 };
-enum : uint32_t { KQ_BAD_LEN = 1, KQ_BAD_PAGE = 2, KQ_BAD_POS = 4, KQ_NOT_FINITE = 8 };
+enum : uint32_t { KQ_BAD_LEN = 1, KQ_BAD_PAGE = 2, KQ_BAD_POS = 4, KQ_NOT_FINITE = 8, KQ_TIMEOUT = 16 };
 // Device view of an fz_kvq8_seqs: sequence i holds lens[i] + len_add positions
 // (lens null: len_add), its last starts[i + 1] - starts[i] (starts null:
 // max_new) are the call's rows; pages null: page j of sequence i is i *

@@ -166,6 +166,7 @@ int fz_kvq8_status(const fz_kvq8* kv, void* stream) {
     if (!bits) return;
     ck(cudaMemsetAsync(c.status, 0, 4, s), "cudaMemsetAsync");
     ck(cudaStreamSynchronize(s), "cudaStreamSynchronize");
+    if (bits & KQ_TIMEOUT) fail(FZ_ETIMEOUT, "8-bit KV cache: a bounded device wait ran out");
     fail(FZ_EINVAL, "8-bit KV cache:%s%s%s%s", bits & KQ_BAD_LEN ? " lengths or rows out of range;" : "",
          bits & KQ_BAD_PAGE ? " page number out of range;" : "",
          bits & KQ_BAD_POS ? " position beyond the rotation table;" : "",

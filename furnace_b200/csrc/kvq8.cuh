@@ -792,6 +792,458 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 }
 
 // ---------------------------------------------------------------------------
+// Attention of many rows (k_kvq8_rows): prompts, and pieces of them, on the
+// fifth-generation tensor cores.
+//
+// A CTA takes 128 rows (row = (new token, query head of the KV head)) and walks
+// the pages they see, one page of 64 positions a step:
+//   warps 4-6  turn the page's codes into fp16 operands in shared memory
+//              (UMMA K-major without swizzle: keys [position][dim], values
+//              [dim][position]); the codes are loaded a step ahead
+//   warp 7     one thread issues S = Q K^T, then O += P V (tcgen05.mma, M = 128)
+//   warps 0-3  a thread a row: scores from tensor memory, softmax, weights back
+// Two CTAs share an SM, so that one's softmax runs under the other's products.
+//
+// The products keep f32's precision as in k_kvq8_split: codes are exact in
+// fp16, and Q and P are two fp16 parts each (Q's rows scaled to 2^13, P's
+// weights by 2^6, so that the low part needs no scale of its own), multiplied
+// one after the other into the same accumulator.  S is double buffered, and a
+// step's P takes the place of its S: 64 columns for the high and the low parts
+// of 64 positions.  P's positions go in the order of the value bytes (2t, 2t +
+// 1, 8 + 2t, 9 + 2t for t = 0..3 of a block), which makes its pairs neighbours
+// and the conversion of the values a plain copy.
+// ---------------------------------------------------------------------------
+constexpr uint32_t KR_M = 128;
+constexpr uint32_t KR_THREADS = 256;  // 128 registers a thread with two CTAs
+constexpr uint32_t KR_CONV = 3;       // warps that convert
+constexpr float KR_P = 64.f;        // scale of the weights
+constexpr uint32_t KR_TMEM = 256;   // columns: S 2 x 64, O HD
+enum : uint32_t { KR_S = 0, KR_O = 128 };
+
+template <int HD>
+struct KrSmem {
+  __half qh[KR_M * HD], ql[KR_M * HD], k[KQ_PAGE * HD], v[KQ_PAGE * HD];
+  float rowf[KR_M];
+  uint32_t rowpos[KR_M];
+  // p_full: two, since a warp may be a step ahead of another
+  uint64_t k_full, v_full, s_full[2], p_full[2], pv_done, fin;
+  uint32_t tmem;
+};
+
+template <uint32_t N>
+__host__ __device__ constexpr uint32_t kr_idesc() {  // f16 x f16 -> f32, M = 128
+  return (1u << 4) | ((N >> 3) << 17) | ((KR_M >> 4) << 24);
+}
+__device__ __forceinline__ void kr_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void kr_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void kr_ld16(uint32_t t, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void kr_st16(uint32_t t, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(t),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void kr_st8(uint32_t t, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void kr_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void kr_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bits n of positions base .. base + 31 with lo <= base + n < hi.
+__device__ __forceinline__ uint32_t kr_bits(uint32_t base, uint32_t lo, uint32_t hi) {
+  const uint32_t a = lo > base ? min(lo - base, 32u) : 0u, b = hi > base ? min(hi - base, 32u) : 0u;
+  const uint32_t below_b = b >= 32 ? 0xffffffffu : (1u << b) - 1, below_a = a >= 32 ? 0xffffffffu : (1u << a) - 1;
+  return below_b & ~below_a;
+}
+
+// One row's step: scores s (64 positions of a page) to the two parts of its
+// weights, which replace them in tensor memory at t.  f and v are the blocks'
+// factors (score, weight); vis: the positions the row sees (MASK).
+struct KrRow {
+  float m = -INFINITY, l = 0.f;
+};
+template <bool MASK>
+__device__ __forceinline__ float kr_top(const float* s, const float* f, const float* v, const uint32_t* vis) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < 4; b++) {
+    float x = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      const int n = b * 16 + k;
+      if (!MASK || (vis[n >> 5] >> (n & 31) & 1)) x = fmaxf(x, s[n]);
+    }
+    if (!MASK || x != -INFINITY) top = fmaxf(top, fmaf(x, f[b], __log2f(fmaxf(v[b], KQ_MIN_SCALE))));
+  }
+  return top;
+}
+template <bool MASK>
+__device__ __forceinline__ void kr_weights(float* s, const float* f, const float* v, const uint32_t* vis, KrRow& r,
+                                           uint32_t t) {
+  const float m = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+  for (int b = 0; b < 4; b++) {
+    float* x = s + 16 * b;
+    const float w = v[b] * KR_P;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+      const int n = b * 16 + k;
+      float e = kq_exp2(fmaf(x[k], f[b], -m));
+      if (MASK && !(vis[n >> 5] >> (n & 31) & 1)) e = 0.f;
+      r.l += e;
+      x[k] = e * w;
+      if (MASK && !(vis[n >> 5] >> (n & 31) & 1)) x[k] = 0.f;  // whatever the scale of a block not written yet
+    }
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++) {  // pair c of the value order: positions 8 (c % 2) + 2 (c / 2), + 1
+      const float a = x[8 * (c & 1) + (c & ~1)], z = x[8 * (c & 1) + (c & ~1) + 1];
+      const __half2 h = __floats2half2_rn(a, z);
+      const float2 g = __half22float2(h);
+      hi[c] = *reinterpret_cast<const uint32_t*>(&h);
+      lo[c] = kq_pack(a - g.x, z - g.y);
+    }
+    kr_st8(t + 8 * b, hi);
+    kr_st8(t + 32 + 8 * b, lo);
+  }
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_constant__ KqSplitArgs<HD, T> a) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  KrSmem<HD>& sm = *reinterpret_cast<KrSmem<HD>*>(smem_raw);
+  constexpr uint32_t half = HD / 2, KJ = HD / 64;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, seq = blockIdx.z;
+  pdl_wait();
+  pdl_trigger();
+  const KqSeq s = kq_plan(a.c, a.b, seq, 0, 0).s;
+  const uint32_t nrows = (uint32_t)s.n_new * a.c.group, tiles = (nrows + KR_M - 1) / KR_M;
+  if (blockIdx.x >= tiles) return;
+  const uint32_t r0 = (tiles - 1 - blockIdx.x) * KR_M;  // the longest first
+  const uint32_t p0 = s.len - s.n_new;
+  const uint32_t plo = p0 + r0 / a.c.group, phi = p0 + min(r0 + KR_M - 1, nrows - 1) / a.c.group;
+  const KqSpan span = kq_span(plo, phi, a.window, a.sinks);
+  auto page_of = [&](uint32_t i) {
+    return (uint32_t)max(kq_page(a.c, a.b, seq, span.page(min(i, span.n - 1))), 0);
+  };
+
+  if (tid == 0) {
+    mbar_init(&sm.k_full, KR_CONV);
+    mbar_init(&sm.v_full, KR_CONV);
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
+    mbar_init(&sm.p_full[0], KR_M);
+    mbar_init(&sm.p_full[1], KR_M);
+    mbar_init(&sm.pv_done, 1);
+    mbar_init(&sm.fin, 1);
+    fence_barrier_init();
+  }
+  if (warp == 7) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                 "n"(KR_TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // the rows, rotated, scaled to 2^13 and split, 16 threads a row
+  {
+    constexpr uint32_t N = half / 16;
+    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {
+      const uint32_t rr = r0 + r, j = rr / a.c.group, l16 = tid & 15, d = l16 * N;
+      float x[2 * N] = {}, top = 0.f;
+      if (rr < nrows) {
+        const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d;
+        kq_ldn<N>(p, x);
+        kq_ldn<N>(p + half, x + N);
+        if (a.c.rope) {
+          float f[2 * N];
+          const float* cs = reinterpret_cast<const float*>(a.c.rope + (uint64_t)(p0 + j) * half + d);
+          kq_ldn<N>(cs, f);
+          kq_ldn<N>(cs + N, f + N);
+#pragma unroll
+          for (uint32_t i = 0; i < N; i++) {
+            const float u = x[i], w = x[N + i];
+            x[i] = __fsub_rn(__fmul_rn(u, f[2 * i]), __fmul_rn(w, f[2 * i + 1]));
+            x[N + i] = __fadd_rn(__fmul_rn(u, f[2 * i + 1]), __fmul_rn(w, f[2 * i]));
+          }
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 2 * N; i++) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int e = max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
+      // a negative softmax scale turns the row, so that factors are not negative
+      const float up = copysignf(__uint_as_float((uint32_t)(127 + 13 - e) << 23), a.scale);
+#pragma unroll
+      for (uint32_t k = 0; k < 2; k++)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i += 2) {
+          const uint32_t at = panel_elem(KR_M, r, k * half + d + i);
+          const float u = x[k * N + i] * up, w = x[k * N + i + 1] * up;
+          const __half2 h = __floats2half2_rn(u, w);
+          const float2 g = __half22float2(h);
+          *reinterpret_cast<__half2*>(&sm.qh[at]) = h;
+          *reinterpret_cast<uint32_t*>(&sm.ql[at]) = kq_pack(u - g.x, w - g.y);
+        }
+      if (l16 == 0) {
+        sm.rowf[r] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+        sm.rowpos[r] = rr < nrows ? p0 + j : phi;  // a row that is none: zeros, not written
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sm.tmem;
+  bool ok = true;
+
+  if (warp == 7) {
+    if (lane == 0) {
+      auto scores = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t part = 0; part < 2; part++)
+#pragma unroll
+          for (uint32_t ks = 0; ks < HD / 16; ks++)
+            kr_mma_ss(tm + KR_S + (i & 1) * KQ_PAGE,
+                      umma_desc((part ? sm.ql : sm.qh) + ks * 2 * (KR_M / 8) * 64, (KR_M / 8) * 128, 128),
+                      umma_desc(sm.k + ks * 2 * (KQ_PAGE / 8) * 64, (KQ_PAGE / 8) * 128, 128), kr_idesc<KQ_PAGE>(),
+                      part || ks);
+        umma_commit(&sm.s_full[i & 1]);
+      };
+      ok = mbar_wait(&sm.k_full, 0);
+      tc_fence_after();
+      if (ok) scores(0);
+      for (uint32_t i = 0; i < span.n && ok; i++) {
+        if (i + 1 < span.n) {
+          ok = mbar_wait(&sm.k_full, (i + 1) & 1) && (i == 0 || mbar_wait(&sm.pv_done, (i - 1) & 1));
+          tc_fence_after();
+          if (ok) scores(i + 1);
+        }
+        ok = ok && mbar_wait(&sm.v_full, i & 1) && mbar_wait(&sm.p_full[i & 1], (i >> 1) & 1);
+        tc_fence_after();
+        if (!ok) break;
+#pragma unroll
+        for (uint32_t part = 0; part < 2; part++)
+#pragma unroll
+          for (uint32_t ks = 0; ks < KQ_PAGE / 16; ks++)
+            kr_mma_ts(tm + KR_O, tm + KR_S + (i & 1) * KQ_PAGE + part * 32 + ks * 8,
+                      umma_desc(sm.v + ks * 2 * (HD / 8) * 64, (HD / 8) * 128, 128), kr_idesc<HD>(),
+                      i || part || ks);
+        umma_commit(&sm.pv_done);
+      }
+      umma_commit(&sm.fin);  // everything issued, whether or not a wait ran out
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const uint32_t cw = warp - 4, g = lane & 7;
+    // 512-byte tiles of a page's side, taken in turn by the warps: 8 KJ of keys,
+    // 4 KJ pairs of values
+    constexpr uint32_t NK = 8 * KJ, NP = 4 * KJ, KX = (NK + KR_CONV - 1) / KR_CONV, VX = (NP + KR_CONV - 1) / KR_CONV;
+    uint4 kr[KX], vr[2 * VX];
+    // the lane's pieces: keys of position g of the tile's 8, dims 16 t .. (t =
+    // lane / 8); values of pieces t = 2 tp, 2 tp + 1 (tp = lane / 8 % 2) of the
+    // pair's tile lane / 16
+    auto load_k = [&](uint32_t page) {
+      const uint8_t* src = a.c.codes + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_PAGE * HD + g * 64 + (lane >> 3) * 16;
+#pragma unroll
+      for (uint32_t x = 0; x < KX; x++)
+        if (cw + KR_CONV * x < NK) kr[x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 512));
+    };
+    auto load_v = [&](uint32_t page) {
+      const uint8_t* src = a.c.codes + (((uint64_t)page * a.c.nkv + kvh) * 2 + 1) * KQ_PAGE * HD + g * 64 +
+                           (lane >> 4) * 512 + (lane >> 3 & 1) * 32;
+#pragma unroll
+      for (uint32_t x = 0; x < VX; x++)
+        if (cw + KR_CONV * x < NP) {
+          vr[2 * x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 1024));
+          vr[2 * x + 1] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 1024 + 16));
+        }
+    };
+    auto put_k = [&]() {
+#pragma unroll
+      for (uint32_t x = 0; x < KX; x++) {
+        const uint32_t tile = cw + KR_CONV * x, tg = tile / KJ, kc = (tile % KJ * 4 + (lane >> 3)) * 2;
+        if (tile >= NK) continue;
+        uint32_t h[8];
+        kq_halves(kr[x].x, h);
+        kq_halves(kr[x].y, h + 2);
+        kq_halves(kr[x].z, h + 4);
+        kq_halves(kr[x].w, h + 6);
+        __half* at = sm.k + (kc * (KQ_PAGE / 8) + tg) * 64 + g * 8;
+        *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(at + (KQ_PAGE / 8) * 64) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    };
+    auto put_v = [&]() {
+#pragma unroll
+      for (uint32_t x = 0; x < VX; x++) {
+        if (cw + KR_CONV * x >= NP) continue;
+        const uint32_t tile = 2 * (cw + KR_CONV * x) + (lane >> 4), blk = tile / (HD / 32), q = tile % (HD / 32);
+        const uint32_t kc = blk * 2 + (lane >> 3 & 1);
+        const uint32_t wa[4] = {vr[2 * x].x, vr[2 * x].y, vr[2 * x].z, vr[2 * x].w};
+        const uint32_t wb[4] = {vr[2 * x + 1].x, vr[2 * x + 1].y, vr[2 * x + 1].z, vr[2 * x + 1].w};
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+          uint32_t h[4];
+          kq_halves(wa[i], h);
+          kq_halves(wb[i], h + 2);
+          *reinterpret_cast<uint4*>(sm.v + (kc * (HD / 8) + q * 4 + i) * 64 + g * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      }
+    };
+    auto full = [&](uint64_t* bar) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    uint32_t page = page_of(0), next = page_of(1);
+    load_k(page);
+    load_v(page);
+    put_k();
+    full(&sm.k_full);
+    load_k(next);
+    // keys run a step ahead of the values: S of the next step is wanted first
+    for (uint32_t i = 0; i < span.n && ok; i++) {
+      const uint32_t after = page_of(i + 2);
+      if (i + 1 < span.n) {
+        ok = mbar_wait(&sm.s_full[i & 1], (i >> 1) & 1);  // S of step i has read the keys
+        if (!ok) break;
+        put_k();
+        full(&sm.k_full);
+        load_k(after);
+      }
+      if (i) ok = mbar_wait(&sm.pv_done, (i - 1) & 1);  // step i - 1 has read the values
+      if (!ok) break;
+      put_v();
+      full(&sm.v_full);
+      load_v(next);
+      next = after;
+    }
+  } else {
+    const uint32_t row = tid, lanes = (warp * 32) << 16;
+    const float rowf = sm.rowf[row];
+    const uint32_t rowpos = sm.rowpos[row];
+    KrRow r;
+    auto scales = [&](uint32_t page, float4* k4, float4* v4) {
+      const float4* p = reinterpret_cast<const float4*>(a.c.scales + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_NB);
+      *k4 = __ldg(p);
+      *v4 = __ldg(p + 1);
+    };
+    float4 k4, v4;
+    scales(page_of(0), &k4, &v4);
+    uint32_t next = page_of(1);
+    for (uint32_t i = 0; i < span.n; i++) {
+      const float f[4] = {k4.x * rowf, k4.y * rowf, k4.z * rowf, k4.w * rowf}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+      scales(next, &k4, &v4);
+      next = page_of(i + 2);
+      ok = mbar_wait(&sm.s_full[i & 1], (i >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t = tm + lanes + KR_S + (i & 1) * KQ_PAGE;
+      float x[64];
+#pragma unroll
+      for (int b = 0; b < 4; b++) kr_ld16(t + 16 * b, x + 16 * b);
+      kr_wait_ld();
+      const uint32_t pos = span.page(i) * KQ_PAGE;
+      const bool masked = pos + KQ_PAGE - 1 > plo || (a.window && pos + KQ_PAGE > a.sinks && phi - min(pos, phi) >= a.window);
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+      float top;
+      if (masked) {
+#pragma unroll
+        for (uint32_t w = 0; w < 2; w++) {
+          const uint32_t base = pos + 32 * w, end = rowpos + 1, from = a.window && end > a.window ? end - a.window : 0;
+          vis[w] = kr_bits(base, from, end);
+          if (a.window) vis[w] |= kr_bits(base, 0, min(a.sinks, end));
+        }
+        top = kr_top<true>(x, f, v, vis);
+      } else {
+        top = kr_top<false>(x, f, v, vis);
+      }
+      if (__any_sync(0xffffffffu, top > r.m + KQ_LAG)) {
+        const float mn = fmaxf(r.m, top), c = mn == r.m ? 1.f : kq_exp2(r.m - mn);
+        r.m = mn;
+        r.l *= c;
+        if (i) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sm.pv_done, (i - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (uint32_t d = 0; d < HD; d += 16) {
+            float o[16];
+            kr_ld16(tm + lanes + KR_O + d, o);
+            kr_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] *= c;
+            kr_st16(tm + lanes + KR_O + d, o);
+          }
+        }
+      }
+      if (masked)
+        kr_weights<true>(x, f, v, vis, r, t);
+      else
+        kr_weights<false>(x, f, v, vis, r, t);
+      kr_wait_st();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[i & 1]);
+    }
+    // the rows' results
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.fin, 0));
+    if (ok) {
+      tc_fence_after();
+      const uint32_t rr = r0 + row;
+      const float inv = r.l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, r.l);
+      T* out = a.out + (uint64_t)(s.row0 + rr / a.c.group) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD;
+#pragma unroll 1
+      for (uint32_t d = 0; d < HD; d += 16) {
+        float o[16];
+        kr_ld16(tm + lanes + KR_O + d, o);
+        kr_wait_ld();
+        if (rr < nrows) {
+#pragma unroll
+          for (int k = 0; k < 16; k++) o[k] = r.l == 0.f ? 0.f : o[k] * inv;
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) kq_st4(out + d + k, o + k);
+        }
+      }
+    }
+  }
+  if (!ok && lane == 0) atomicOr(a.c.status, KQ_TIMEOUT);
+  if (tid == 224) mbar_wait(&sm.fin, 0);  // nothing of this CTA's is in flight
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 7)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(KR_TMEM) : "memory");
+}
+
+// ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
 template <int HD, typename T>
@@ -844,6 +1296,14 @@ static uint32_t kvq8_runs(const KvQ8Dev& c, const KvQ8Batch& b) {
 }
 static uint64_t kvq8_prefix_bytes(const KvQ8Batch& b) { return ((uint64_t)b.n_seqs + 1) * 8 + 15 & ~15ull; }
 
+// Many rows go to k_kvq8_rows.  It reads a page once for 128 rows, but a
+// sequence's rows walk all their pages one after the other, so there have to
+// be row groups enough for the split form to take longer.
+static bool kvq8_by_rows(const KvQ8Dev& c, const KvQ8Batch& b) {
+  const uint64_t rows = (uint64_t)b.max_new * c.group;
+  return rows >= 64 && b.n_seqs * c.nkv * ((rows + 7) / 8) >= 256;
+}
+
 uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b) {
   return kvq8_prefix_bytes(b) + 2ull * kvq8_runs(c, b) * (8 * c.hd + 16) * 4;
 }
@@ -855,6 +1315,7 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
   kvq8_once(ready, [&] {
     CK(cudaFuncSetAttribute(k_kvq8_split<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     CK(cudaFuncSetAttribute(k_kvq8_whole<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CK(cudaFuncSetAttribute(k_kvq8_rows<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KrSmem<HD>)));
   });
   const uint32_t runs = kvq8_runs(a.c, a.b);
   KqSplitArgs<HD, T> k{a.c,
@@ -868,6 +1329,11 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
                        a.scale * 1.44269504088896341f,
                        static_cast<uint64_t*>(a.work),
                        reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b))};
+  if (kvq8_by_rows(a.c, a.b)) {
+    const uint32_t tiles = (uint32_t)(((uint64_t)a.b.max_new * a.c.group + KR_M - 1) / KR_M);
+    launch_pdl(k_kvq8_rows<HD, T>, dim3(tiles, a.c.nkv, a.b.n_seqs), dim3(KR_THREADS), sizeof(KrSmem<HD>), s, k);
+    return;
+  }
   if (a.b.max_pages <= KQ_WHOLE_PAGES) {
     const uint64_t groups = ((uint64_t)a.b.max_new * a.c.group + 7) / 8;
     launch_pdl(k_kvq8_whole<HD, T>, dim3((unsigned)(a.c.nkv * groups), a.b.n_seqs), dim3(KQ_SP_THREADS), smem, s, k);
