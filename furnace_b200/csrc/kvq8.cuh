@@ -797,36 +797,40 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 //
 // A CTA takes 128 rows (row = (new token, query head of the KV head)) and walks
 // the pages they see, one page of 64 positions a step:
-//   warps 4-6  turn the page's codes into fp16 operands in shared memory
+//   warps 8-10 turn the page's codes into fp16 operands in shared memory
 //              (UMMA K-major without swizzle: keys [position][dim], values
 //              [dim][position]); the codes are loaded a step ahead
-//   warp 7     one thread issues S = Q K^T, then O += P V (tcgen05.mma, M = 128)
+//   warp 11    one thread issues S = Q K^T, then O = P V (tcgen05.mma, M = 128)
 //   warps 0-3  a thread a row: scores from tensor memory, softmax, weights back
-// Two CTAs share an SM, so that one's softmax runs under the other's products.
+//   warps 4-7  a thread a row: the step's O from tensor memory, added to the
+//              row's sums in registers
 //
 // The products keep f32's precision as in k_kvq8_split: codes are exact in
 // fp16, and Q and P are two fp16 parts each (Q's rows scaled to 2^13, P's
-// weights by 2^6, so that the low part needs no scale of its own), multiplied
-// one after the other into the same accumulator.  S is double buffered, and a
-// step's P takes the place of its S: 64 columns for the high and the low parts
-// of 64 positions.  P's positions go in the order of the value bytes (2t, 2t +
-// 1, 8 + 2t, 9 + 2t for t = 0..3 of a block), which makes its pairs neighbours
-// and the conversion of the values a plain copy.
+// weights by 2^13, so that the low part needs no scale of its own), multiplied
+// one after the other into the same accumulator.  The tensor cores' additions
+// truncate, which loses 1.3e-7 a step where O stays in tensor memory (3.8e-5
+// after 250 pages): hence the sums in registers, and hence one CTA an SM.  S, O
+// and the operands are double buffered, and a step's P takes the place of its
+// S: 64 columns for the high and the low parts of 64 positions.  P's positions
+// go in the order of the value bytes (2t, 2t + 1, 8 + 2t, 9 + 2t for t = 0..3 of
+// a block), which makes its pairs neighbours and the conversion of the values
+// a plain copy.
 // ---------------------------------------------------------------------------
 constexpr uint32_t KR_M = 128;
-constexpr uint32_t KR_THREADS = 256;  // 128 registers a thread with two CTAs
-constexpr uint32_t KR_CONV = 3;       // warps that convert
-constexpr float KR_P = 64.f;        // scale of the weights
-constexpr uint32_t KR_TMEM = 256;   // columns: S 2 x 64, O HD
-enum : uint32_t { KR_S = 0, KR_O = 128 };
+constexpr uint32_t KR_THREADS = 384;  // 168 registers a thread
+constexpr uint32_t KR_CONV = 3;     // warps that convert
+constexpr float KR_P = 8192.f;      // scale of the weights
+enum : uint32_t { KR_S = 0, KR_O = 128 };  // tensor memory: S 2 x 64 columns, O 2 x HD
+template <int HD>
+constexpr uint32_t kr_tmem = HD == 128 ? 512 : 256;
 
 template <int HD>
 struct KrSmem {
-  __half qh[KR_M * HD], ql[KR_M * HD], k[KQ_PAGE * HD], v[KQ_PAGE * HD];
-  float rowf[KR_M];
+  __half qh[KR_M * HD], ql[KR_M * HD], k[2][KQ_PAGE * HD], v[2][KQ_PAGE * HD];
+  float rowf[KR_M], l[KR_M], alpha[2][KR_M];
   uint32_t rowpos[KR_M];
-  // p_full: two, since a warp may be a step ahead of another
-  uint64_t k_full, v_full, s_full[2], p_full[2], pv_done, fin;
+  uint64_t k_full[2], v_full[2], s_full[2], p_full[2], o_full[2], o_free[2], l_full, fin;
   uint32_t tmem;
 };
 
@@ -858,21 +862,20 @@ __device__ __forceinline__ void kr_ld16(uint32_t t, float* v) {
       : "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void kr_st16(uint32_t t, const float* v) {
-  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(t),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 __device__ __forceinline__ void kr_st8(uint32_t t, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void kr_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Wait for the loads; the registers go through it, so that nothing that uses
+// them comes before it.
+__device__ __forceinline__ void kr_wait_ld(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void kr_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bits n of positions base .. base + 31 with lo <= base + n < hi.
@@ -935,7 +938,7 @@ __device__ __forceinline__ void kr_weights(float* s, const float* f, const float
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_constant__ KqSplitArgs<HD, T> a) {
+__global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_constant__ KqSplitArgs<HD, T> a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   KrSmem<HD>& sm = *reinterpret_cast<KrSmem<HD>*>(smem_raw);
   constexpr uint32_t half = HD / 2, KJ = HD / 64;
@@ -954,26 +957,28 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
   };
 
   if (tid == 0) {
-    mbar_init(&sm.k_full, KR_CONV);
-    mbar_init(&sm.v_full, KR_CONV);
-    mbar_init(&sm.s_full[0], 1);
-    mbar_init(&sm.s_full[1], 1);
-    mbar_init(&sm.p_full[0], KR_M);
-    mbar_init(&sm.p_full[1], KR_M);
-    mbar_init(&sm.pv_done, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sm.k_full[i], KR_CONV);
+      mbar_init(&sm.v_full[i], KR_CONV);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], KR_M);
+      mbar_init(&sm.o_full[i], 1);
+      mbar_init(&sm.o_free[i], KR_M);
+    }
+    mbar_init(&sm.l_full, KR_M);
     mbar_init(&sm.fin, 1);
     fence_barrier_init();
   }
-  if (warp == 7) {
+  if (warp == 11) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
-                 "n"(KR_TMEM)
+                 "n"(kr_tmem<HD>)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // the rows, rotated, scaled to 2^13 and split, 16 threads a row
   {
     constexpr uint32_t N = half / 16;
-    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {
+    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {  // whole warps: 24 rows a pass
       const uint32_t rr = r0 + r, j = rr / a.c.group, l16 = tid & 15, d = l16 * N;
       float x[2 * N] = {}, top = 0.f;
       if (rr < nrows) {
@@ -1024,7 +1029,11 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
   const uint32_t tm = sm.tmem;
   bool ok = true;
 
-  if (warp == 7) {
+  // Step i uses buffer i % 2 of everything, for the (i / 2)th time: a wait for
+  // step i's use is a wait for parity (i / 2) % 2.
+  auto wait = [&](uint64_t* bar, uint32_t i) { return mbar_wait(&bar[i & 1], (i >> 1) & 1); };
+
+  if (warp == 11) {
     if (lane == 0) {
       auto scores = [&](uint32_t i) {
 #pragma unroll
@@ -1033,36 +1042,37 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
           for (uint32_t ks = 0; ks < HD / 16; ks++)
             kr_mma_ss(tm + KR_S + (i & 1) * KQ_PAGE,
                       umma_desc((part ? sm.ql : sm.qh) + ks * 2 * (KR_M / 8) * 64, (KR_M / 8) * 128, 128),
-                      umma_desc(sm.k + ks * 2 * (KQ_PAGE / 8) * 64, (KQ_PAGE / 8) * 128, 128), kr_idesc<KQ_PAGE>(),
-                      part || ks);
+                      umma_desc(sm.k[i & 1] + ks * 2 * (KQ_PAGE / 8) * 64, (KQ_PAGE / 8) * 128, 128),
+                      kr_idesc<KQ_PAGE>(), part || ks);
         umma_commit(&sm.s_full[i & 1]);
       };
-      ok = mbar_wait(&sm.k_full, 0);
+      ok = wait(sm.k_full, 0);
       tc_fence_after();
       if (ok) scores(0);
       for (uint32_t i = 0; i < span.n && ok; i++) {
-        if (i + 1 < span.n) {
-          ok = mbar_wait(&sm.k_full, (i + 1) & 1) && (i == 0 || mbar_wait(&sm.pv_done, (i - 1) & 1));
+        if (i + 1 < span.n) {  // S of the next step replaces P of the last
+          ok = wait(sm.k_full, i + 1) && (i == 0 || wait(sm.o_full, i - 1));
           tc_fence_after();
           if (ok) scores(i + 1);
         }
-        ok = ok && mbar_wait(&sm.v_full, i & 1) && mbar_wait(&sm.p_full[i & 1], (i >> 1) & 1);
+        ok = ok && wait(sm.v_full, i) && wait(sm.p_full, i) && (i < 2 || wait(sm.o_free, i - 2));
         tc_fence_after();
         if (!ok) break;
 #pragma unroll
         for (uint32_t part = 0; part < 2; part++)
 #pragma unroll
           for (uint32_t ks = 0; ks < KQ_PAGE / 16; ks++)
-            kr_mma_ts(tm + KR_O, tm + KR_S + (i & 1) * KQ_PAGE + part * 32 + ks * 8,
-                      umma_desc(sm.v + ks * 2 * (HD / 8) * 64, (HD / 8) * 128, 128), kr_idesc<HD>(),
-                      i || part || ks);
-        umma_commit(&sm.pv_done);
+            kr_mma_ts(tm + KR_O + (i & 1) * HD, tm + KR_S + (i & 1) * KQ_PAGE + part * 32 + ks * 8,
+                      umma_desc(sm.v[i & 1] + ks * 2 * (HD / 8) * 64, (HD / 8) * 128, 128), kr_idesc<HD>(),
+                      part || ks);
+        umma_commit(&sm.o_full[i & 1]);
       }
       umma_commit(&sm.fin);  // everything issued, whether or not a wait ran out
+      mbar_wait(&sm.fin, 0);
     }
     __syncwarp();
-  } else if (warp >= 4) {
-    const uint32_t cw = warp - 4, g = lane & 7;
+  } else if (warp >= 8) {
+    const uint32_t cw = warp - 8, g = lane & 7;
     // 512-byte tiles of a page's side, taken in turn by the warps: 8 KJ of keys,
     // 4 KJ pairs of values
     constexpr uint32_t NK = 8 * KJ, NP = 4 * KJ, KX = (NK + KR_CONV - 1) / KR_CONV, VX = (NP + KR_CONV - 1) / KR_CONV;
@@ -1086,7 +1096,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
           vr[2 * x + 1] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 1024 + 16));
         }
     };
-    auto put_k = [&]() {
+    auto put_k = [&](__half* dst) {
 #pragma unroll
       for (uint32_t x = 0; x < KX; x++) {
         const uint32_t tile = cw + KR_CONV * x, tg = tile / KJ, kc = (tile % KJ * 4 + (lane >> 3)) * 2;
@@ -1096,12 +1106,12 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
         kq_halves(kr[x].y, h + 2);
         kq_halves(kr[x].z, h + 4);
         kq_halves(kr[x].w, h + 6);
-        __half* at = sm.k + (kc * (KQ_PAGE / 8) + tg) * 64 + g * 8;
+        __half* at = dst + (kc * (KQ_PAGE / 8) + tg) * 64 + g * 8;
         *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(at + (KQ_PAGE / 8) * 64) = make_uint4(h[4], h[5], h[6], h[7]);
       }
     };
-    auto put_v = [&]() {
+    auto put_v = [&](__half* dst) {
 #pragma unroll
       for (uint32_t x = 0; x < VX; x++) {
         if (cw + KR_CONV * x >= NP) continue;
@@ -1114,7 +1124,7 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
           uint32_t h[4];
           kq_halves(wa[i], h);
           kq_halves(wb[i], h + 2);
-          *reinterpret_cast<uint4*>(sm.v + (kc * (HD / 8) + q * 4 + i) * 64 + g * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + (kc * (HD / 8) + q * 4 + i) * 64 + g * 8) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
     };
@@ -1123,28 +1133,55 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    uint32_t page = page_of(0), next = page_of(1);
-    load_k(page);
-    load_v(page);
-    put_k();
-    full(&sm.k_full);
+    uint32_t next = page_of(0);
     load_k(next);
-    // keys run a step ahead of the values: S of the next step is wanted first
-    for (uint32_t i = 0; i < span.n && ok; i++) {
-      const uint32_t after = page_of(i + 2);
-      if (i + 1 < span.n) {
-        ok = mbar_wait(&sm.s_full[i & 1], (i >> 1) & 1);  // S of step i has read the keys
-        if (!ok) break;
-        put_k();
-        full(&sm.k_full);
-        load_k(after);
-      }
-      if (i) ok = mbar_wait(&sm.pv_done, (i - 1) & 1);  // step i - 1 has read the values
+    load_v(next);
+    next = page_of(1);
+    for (uint32_t i = 0; i < span.n; i++) {
+      ok = i < 2 || wait(sm.s_full, i - 2);  // S of step i - 2 has read the keys
       if (!ok) break;
-      put_v();
-      full(&sm.v_full);
+      put_k(sm.k[i & 1]);
+      full(&sm.k_full[i & 1]);
+      load_k(next);
+      ok = i < 2 || wait(sm.o_full, i - 2);  // its O the values
+      if (!ok) break;
+      put_v(sm.v[i & 1]);
+      full(&sm.v_full[i & 1]);
       load_v(next);
-      next = after;
+      next = page_of(i + 2);
+    }
+  } else if (warp >= 4) {
+    const uint32_t row = tid - 128, lanes = ((warp & 3) * 32) << 16;
+    float acc[HD];
+#pragma unroll
+    for (int d = 0; d < HD; d++) acc[d] = 0.f;
+    for (uint32_t i = 0; i < span.n; i++) {
+      ok = __all_sync(0xffffffffu, wait(sm.p_full, i) && wait(sm.o_full, i));
+      if (!ok) break;
+      tc_fence_after();
+      const float alpha = sm.alpha[i & 1][row];
+#pragma unroll
+      for (int d = 0; d < HD; d += 16) {
+        float o[16];
+        kr_ld16(tm + lanes + KR_O + (i & 1) * HD + d, o);
+        kr_wait_ld(o);
+#pragma unroll
+        for (int k = 0; k < 16; k++) acc[d + k] = fmaf(acc[d + k], alpha, o[k]);
+      }
+      tc_fence_before();
+      mbar_arrive(&sm.o_free[i & 1]);
+    }
+    ok = ok && mbar_wait(&sm.l_full, 0);
+    const uint32_t rr = r0 + row;
+    if (ok && rr < nrows) {
+      const float l = sm.l[row], inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
+      T* out = a.out + (uint64_t)(s.row0 + rr / a.c.group) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD;
+#pragma unroll
+      for (int d = 0; d < HD; d += 4) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) acc[d + k] = l == 0.f ? 0.f : acc[d + k] * inv;
+        kq_st4(out + d, acc + d);
+      }
     }
   } else {
     const uint32_t row = tid, lanes = (warp * 32) << 16;
@@ -1163,15 +1200,15 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
       const float f[4] = {k4.x * rowf, k4.y * rowf, k4.z * rowf, k4.w * rowf}, v[4] = {v4.x, v4.y, v4.z, v4.w};
       scales(next, &k4, &v4);
       next = page_of(i + 2);
-      ok = mbar_wait(&sm.s_full[i & 1], (i >> 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, wait(sm.s_full, i));
       if (!ok) break;
       tc_fence_after();
       const uint32_t t = tm + lanes + KR_S + (i & 1) * KQ_PAGE;
       float x[64];
 #pragma unroll
       for (int b = 0; b < 4; b++) kr_ld16(t + 16 * b, x + 16 * b);
-      kr_wait_ld();
+#pragma unroll
+      for (int b = 0; b < 4; b++) kr_wait_ld(x + 16 * b);
       const uint32_t pos = span.page(i) * KQ_PAGE;
       const bool masked = pos + KQ_PAGE - 1 > plo || (a.window && pos + KQ_PAGE > a.sinks && phi - min(pos, phi) >= a.window);
       uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
@@ -1187,60 +1224,29 @@ __global__ void __launch_bounds__(KR_THREADS, 2) k_kvq8_rows(const __grid_consta
       } else {
         top = kr_top<false>(x, f, v, vis);
       }
-      if (__any_sync(0xffffffffu, top > r.m + KQ_LAG)) {
-        const float mn = fmaxf(r.m, top), c = mn == r.m ? 1.f : kq_exp2(r.m - mn);
-        r.m = mn;
-        r.l *= c;
-        if (i) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&sm.pv_done, (i - 1) & 1));
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (uint32_t d = 0; d < HD; d += 16) {
-            float o[16];
-            kr_ld16(tm + lanes + KR_O + d, o);
-            kr_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; k++) o[k] *= c;
-            kr_st16(tm + lanes + KR_O + d, o);
-          }
-        }
-      }
+      const float mn = fmaxf(r.m, top), c = mn == r.m ? 1.f : kq_exp2(r.m - mn);
+      r.m = mn;
+      r.l *= c;
       if (masked)
         kr_weights<true>(x, f, v, vis, r, t);
       else
         kr_weights<false>(x, f, v, vis, r, t);
       kr_wait_st();
+      ok = i < 2 || wait(sm.o_free, i - 2);  // alpha of step i - 2 has been read
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      sm.alpha[i & 1][row] = c;
       tc_fence_before();
       mbar_arrive(&sm.p_full[i & 1]);
     }
-    // the rows' results
-    ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.fin, 0));
-    if (ok) {
-      tc_fence_after();
-      const uint32_t rr = r0 + row;
-      const float inv = r.l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, r.l);
-      T* out = a.out + (uint64_t)(s.row0 + rr / a.c.group) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD;
-#pragma unroll 1
-      for (uint32_t d = 0; d < HD; d += 16) {
-        float o[16];
-        kr_ld16(tm + lanes + KR_O + d, o);
-        kr_wait_ld();
-        if (rr < nrows) {
-#pragma unroll
-          for (int k = 0; k < 16; k++) o[k] = r.l == 0.f ? 0.f : o[k] * inv;
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) kq_st4(out + d + k, o + k);
-        }
-      }
-    }
+    sm.l[row] = r.l;
+    mbar_arrive(&sm.l_full);
   }
   if (!ok && lane == 0) atomicOr(a.c.status, KQ_TIMEOUT);
-  if (tid == 224) mbar_wait(&sm.fin, 0);  // nothing of this CTA's is in flight
   tc_fence_before();
   __syncthreads();
-  if (warp == 7)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(KR_TMEM) : "memory");
+  if (warp == 11)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kr_tmem<HD>) : "memory");
 }
 
 // ---------------------------------------------------------------------------
