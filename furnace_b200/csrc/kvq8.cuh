@@ -796,41 +796,51 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 // fifth-generation tensor cores.
 //
 // A CTA takes 128 rows (row = (new token, query head of the KV head)) and walks
-// the pages they see, one page of 64 positions a step:
-//   warps 8-10 turn the page's codes into fp16 operands in shared memory
-//              (UMMA K-major without swizzle: keys [position][dim], values
-//              [dim][position]); the codes are loaded a step ahead
-//   warp 11    one thread issues S = Q K^T, then O = P V (tcgen05.mma, M = 128)
-//   warps 0-3  a thread a row: scores from tensor memory, softmax, weights back
-//   warps 4-7  a thread a row: the step's O from tensor memory, added to the
-//              row's sums in registers
+// the pages they see, two pages (128 positions) a step:
+//   warps 0-3    a thread a row, even steps: scores from tensor memory, softmax,
+//   and 4-7      weights back; odd steps
+//   warps 8-11   turn the next step's values into an fp16 operand in shared
+//                memory (UMMA K-major without swizzle, [dim][position]), then,
+//                a thread a row, add the step's O from tensor memory to the
+//                row's sums in registers
+//   warps 12-14  turn the keys into their operand ([position][dim])
+//   warp 15      one thread issues S = Q K^T, then O = P V (tcgen05.mma, M = 128)
 //
 // The products keep f32's precision as in k_kvq8_split: codes are exact in
 // fp16, and Q and P are two fp16 parts each (Q's rows scaled to 2^13, P's
 // weights by 2^13, so that the low part needs no scale of its own), multiplied
-// one after the other into the same accumulator.  The tensor cores' additions
-// truncate, which loses 1.3e-7 a step where O stays in tensor memory (3.8e-5
-// after 250 pages): hence the sums in registers, and hence one CTA an SM.  S, O
-// and the operands are double buffered, and a step's P takes the place of its
-// S: 64 columns for the high and the low parts of 64 positions.  P's positions
-// go in the order of the value bytes (2t, 2t + 1, 8 + 2t, 9 + 2t for t = 0..3 of
-// a block), which makes its pairs neighbours and the conversion of the values
-// a plain copy.
+// one after the other into the same accumulator, the low part first, while
+// what the tensor cores' additions cut off is small.  Over a long run that
+// still adds up (3.8e-5 after 250 pages where O stayed in tensor memory):
+// hence the sums in registers, and hence one CTA an SM.  Two pages a step: a
+// product of 128 positions reads its 128 rows once instead of twice, which
+// bounded it (1200 cycles for the scores of one page).  The two warpgroups of
+// the softmax take turns, so that one's exponentials run under the other's
+// maximum, conversion and waits; the running maximum goes from one to the
+// other as soon as a step's is known.  Scores have three buffers in tensor
+// memory, so that neither waits for the other's products, and a step's P takes
+// the place of its S: of 32 positions, 16 columns for the high and 16 for the
+// low parts.  P's positions go in the order of the value bytes (2t, 2t + 1, 8 +
+// 2t, 9 + 2t for t = 0..3 of a block), which makes its pairs neighbours and the
+// conversion of the values a plain copy.
 // ---------------------------------------------------------------------------
 constexpr uint32_t KR_M = 128;
-constexpr uint32_t KR_THREADS = 384;  // 168 registers a thread
-constexpr uint32_t KR_CONV = 3;     // warps that convert
-constexpr float KR_P = 8192.f;      // scale of the weights
-enum : uint32_t { KR_S = 0, KR_O = 128 };  // tensor memory: S 2 x 64 columns, O 2 x HD
-template <int HD>
-constexpr uint32_t kr_tmem = HD == 128 ? 512 : 256;
+constexpr uint32_t KR_THREADS = 512;
+constexpr uint32_t KR_CONV = 3;            // warps that convert keys
+constexpr uint32_t KR_POS = 2 * KQ_PAGE;   // positions of a step
+constexpr float KR_P = 8192.f;             // scale of the weights
+// registers: 128 a thread at launch, 512 for the four warpgroups together
+constexpr int KR_REG_ACC = 200, KR_REG_OTHER = 104;
+static_assert(3 * KR_REG_OTHER + KR_REG_ACC <= 512, "register shares");
+constexpr uint32_t KR_NS = 3;              // scores in tensor memory
+enum : uint32_t { KR_S = 0, KR_O = KR_NS * KR_POS };  // tensor memory: S 3 x 128 columns, O HD
 
 template <int HD>
 struct KrSmem {
-  __half qh[KR_M * HD], ql[KR_M * HD], k[2][KQ_PAGE * HD], v[2][KQ_PAGE * HD];
-  float rowf[KR_M], l[KR_M], alpha[2][KR_M];
+  __half qh[KR_M * HD], ql[KR_M * HD], k[2][KR_POS * HD], v[2][KR_POS * HD];
+  float rowf[KR_M], l[2][KR_M], last[2][KR_M], m[2][KR_M], alpha[4][KR_M];
   uint32_t rowpos[KR_M];
-  uint64_t k_full[2], v_full[2], s_full[2], p_full[2], o_full[2], o_free[2], l_full, fin;
+  uint64_t k_full[2], v_full[2], s_full[KR_NS], m_full[2], a_full[4], p_full[KR_NS], o_full, o_free, l_full, fin;
   uint32_t tmem;
 };
 
@@ -862,6 +872,19 @@ __device__ __forceinline__ void kr_ld16(uint32_t t, float* v) {
       : "r"(t)
       : "memory");
 }
+__device__ __forceinline__ void kr_ld32(uint32_t t, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+      "[%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t)
+      : "memory");
+}
 __device__ __forceinline__ void kr_st8(uint32_t t, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -878,6 +901,15 @@ __device__ __forceinline__ void kr_wait_ld(float* v) {
 }
 __device__ __forceinline__ void kr_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+template <int N>
+__device__ __forceinline__ void kr_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void kr_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Bits n of positions base .. base + 31 with lo <= base + n < hi.
 __device__ __forceinline__ uint32_t kr_bits(uint32_t base, uint32_t lo, uint32_t hi) {
   const uint32_t a = lo > base ? min(lo - base, 32u) : 0u, b = hi > base ? min(hi - base, 32u) : 0u;
@@ -885,56 +917,71 @@ __device__ __forceinline__ uint32_t kr_bits(uint32_t base, uint32_t lo, uint32_t
   return below_b & ~below_a;
 }
 
-// One row's step: scores s (64 positions of a page) to the two parts of its
-// weights, which replace them in tensor memory at t.  f and v are the blocks'
-// factors (score, weight); vis: the positions the row sees (MASK).
-struct KrRow {
-  float m = -INFINITY, l = 0.f;
+// Page numbers of 32 pages, one per lane, and of the 32 after them.
+struct KrPages {
+  uint32_t cur, next;
+  template <class F>
+  __device__ __forceinline__ KrPages(F&& page_of, uint32_t lane) : cur(page_of(lane)), next(page_of(32 + lane)) {}
+  // before the first use of page n, an even number
+  template <class F>
+  __device__ __forceinline__ void move(F&& page_of, uint32_t lane, uint32_t n) {
+    if (n % 32 == 0) {
+      cur = next;
+      next = page_of(n + 32 + lane);
+    }
+  }
+  __device__ __forceinline__ uint32_t at(uint32_t n) const { return __shfl_sync(0xffffffffu, cur, n % 32); }
 };
+
+// One row and 16 positions (a block) of a step.  f and lv are the block's score
+// factor and the log2 of its value scale, bits the positions that the row sees
+// (MASK).
 template <bool MASK>
-__device__ __forceinline__ float kr_top(const float* s, const float* f, const float* v, const uint32_t* vis) {
-  float top = -INFINITY;
+__device__ __forceinline__ float kr_top(const float* s, float f, float lv, uint32_t bits) {
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int b = 0; b < 4; b++) {
-    float x = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 16; k++) {
-      const int n = b * 16 + k;
-      if (!MASK || (vis[n >> 5] >> (n & 31) & 1)) x = fmaxf(x, s[n]);
-    }
-    if (!MASK || x != -INFINITY) top = fmaxf(top, fmaf(x, f[b], __log2f(fmaxf(v[b], KQ_MIN_SCALE))));
-  }
-  return top;
+  for (int k = 0; k < 16; k++)
+    if (!MASK || (bits >> k & 1)) x[k & 3] = fmaxf(x[k & 3], s[k]);
+  const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  return MASK && top == -INFINITY ? top : fmaf(top, f, lv);
 }
-template <bool MASK>
-__device__ __forceinline__ void kr_weights(float* s, const float* f, const float* v, const uint32_t* vis, KrRow& r,
-                                           uint32_t t) {
-  const float m = r.m == -INFINITY ? 0.f : r.m;
+// Weights to tensor memory at t, the high parts, and t + 16, the low ones.
+__device__ __forceinline__ void kr_put(const float* x, uint32_t t) {
+  uint32_t hi[8], lo[8];
 #pragma unroll
-  for (int b = 0; b < 4; b++) {
-    float* x = s + 16 * b;
-    const float w = v[b] * KR_P;
-#pragma unroll
-    for (int k = 0; k < 16; k++) {
-      const int n = b * 16 + k;
-      float e = kq_exp2(fmaf(x[k], f[b], -m));
-      if (MASK && !(vis[n >> 5] >> (n & 31) & 1)) e = 0.f;
-      r.l += e;
-      x[k] = e * w;
-      if (MASK && !(vis[n >> 5] >> (n & 31) & 1)) x[k] = 0.f;  // whatever the scale of a block not written yet
-    }
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int c = 0; c < 8; c++) {  // pair c of the value order: positions 8 (c % 2) + 2 (c / 2), + 1
-      const float a = x[8 * (c & 1) + (c & ~1)], z = x[8 * (c & 1) + (c & ~1) + 1];
-      const __half2 h = __floats2half2_rn(a, z);
-      const float2 g = __half22float2(h);
-      hi[c] = *reinterpret_cast<const uint32_t*>(&h);
-      lo[c] = kq_pack(a - g.x, z - g.y);
-    }
-    kr_st8(t + 8 * b, hi);
-    kr_st8(t + 32 + 8 * b, lo);
+  for (int c = 0; c < 8; c++) {  // pair c of the value order: positions 8 (c % 2) + 2 (c / 2), + 1
+    const float a = x[8 * (c & 1) + (c & ~1)], z = x[8 * (c & 1) + (c & ~1) + 1];
+    const __half2 h = __floats2half2_rn(a, z);
+    const float2 g = __half22float2(h);
+    hi[c] = *reinterpret_cast<const uint32_t*>(&h);
+    lo[c] = kq_pack(a - g.x, z - g.y);
   }
+  kr_st8(t, hi);
+  kr_st8(t + 16, lo);
+}
+// The block's weights 2^(f s - m) v KR_P: c = log2(v KR_P) - m puts the scale
+// into the exponent, and the denominator is the weights' sum / (v KR_P).
+__device__ __forceinline__ float kr_weights(float* x, float f, float c) {
+  float sum[4] = {};
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    x[k] = kq_exp2(fmaf(x[k], f, c));
+    sum[k & 3] += x[k];
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// The same with positions that the row does not see, and for any scale: w = v
+// KR_P apart from the exponent.  Returns the denominator.
+__device__ __forceinline__ float kr_weights_masked(float* x, float f, float w, float m, uint32_t bits) {
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; k++) {
+    const bool seen = bits >> k & 1;
+    const float e = kq_exp2(fmaf(x[k], f, -m));
+    sum += seen ? e : 0.f;
+    x[k] = seen ? e * w : 0.f;  // 0 whatever the scale of a block not written yet
+  }
+  return sum;
 }
 
 template <int HD, typename T>
@@ -959,26 +1006,29 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&sm.k_full[i], KR_CONV);
-      mbar_init(&sm.v_full[i], KR_CONV);
+      mbar_init(&sm.v_full[i], 4);
+      mbar_init(&sm.m_full[i], KR_M);
+    }
+    for (uint32_t i = 0; i < KR_NS; i++) {
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], KR_M);
-      mbar_init(&sm.o_full[i], 1);
-      mbar_init(&sm.o_free[i], KR_M);
     }
-    mbar_init(&sm.l_full, KR_M);
+    for (int i = 0; i < 4; i++) mbar_init(&sm.a_full[i], KR_M);
+    mbar_init(&sm.o_full, 1);
+    mbar_init(&sm.o_free, KR_M);
+    mbar_init(&sm.l_full, 2 * KR_M);
     mbar_init(&sm.fin, 1);
     fence_barrier_init();
   }
-  if (warp == 11) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
-                 "n"(kr_tmem<HD>)
+  if (warp == 15) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // the rows, rotated, scaled to 2^13 and split, 16 threads a row
   {
     constexpr uint32_t N = half / 16;
-    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {  // whole warps: 24 rows a pass
+    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {  // whole warps
       const uint32_t rr = r0 + r, j = rr / a.c.group, l16 = tid & 15, d = l16 * N;
       float x[2 * N] = {}, top = 0.f;
       if (rr < nrows) {
@@ -1029,152 +1079,176 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   const uint32_t tm = sm.tmem;
   bool ok = true;
 
-  // Step i uses buffer i % 2 of everything, for the (i / 2)th time: a wait for
-  // step i's use is a wait for parity (i / 2) % 2.
-  auto wait = [&](uint64_t* bar, uint32_t i) { return mbar_wait(&bar[i & 1], (i >> 1) & 1); };
+  // With n buffers, step i uses buffer i % n, for the (i / n)th time: a wait for
+  // step i's use is a wait for parity (i / n) % 2.  No barrier may get a whole
+  // use ahead of a thread that still waits for the one before; beside each wait
+  // stands what the next use needs from that thread.
+  auto wait = [&](auto& bar, uint32_t i) {
+    constexpr uint32_t n = sizeof(bar) / sizeof(uint64_t);
+    return mbar_wait(reinterpret_cast<uint64_t*>(&bar) + i % n, (i / n) & 1);
+  };
+  const uint32_t steps = (span.n + 1) / 2;
 
-  if (warp == 11) {
+  if (warp >= 12) kr_regs_dec<KR_REG_OTHER>();
+  if (warp == 15) {
     if (lane == 0) {
       auto scores = [&](uint32_t i) {
-#pragma unroll
+#pragma unroll 1
         for (uint32_t part = 0; part < 2; part++)
 #pragma unroll
           for (uint32_t ks = 0; ks < HD / 16; ks++)
-            kr_mma_ss(tm + KR_S + (i & 1) * KQ_PAGE,
-                      umma_desc((part ? sm.ql : sm.qh) + ks * 2 * (KR_M / 8) * 64, (KR_M / 8) * 128, 128),
-                      umma_desc(sm.k[i & 1] + ks * 2 * (KQ_PAGE / 8) * 64, (KQ_PAGE / 8) * 128, 128),
-                      kr_idesc<KQ_PAGE>(), part || ks);
-        umma_commit(&sm.s_full[i & 1]);
+            kr_mma_ss(tm + KR_S + i % KR_NS * KR_POS,
+                      umma_desc((part ? sm.qh : sm.ql) + ks * 2 * (KR_M / 8) * 64, (KR_M / 8) * 128, 128),
+                      umma_desc(sm.k[i & 1] + ks * 2 * (KR_POS / 8) * 64, (KR_POS / 8) * 128, 128),
+                      kr_idesc<KR_POS>(), part || ks);
+        umma_commit(&sm.s_full[i % KR_NS]);
       };
-      ok = wait(sm.k_full, 0);
-      tc_fence_after();
-      if (ok) scores(0);
-      for (uint32_t i = 0; i < span.n && ok; i++) {
-        if (i + 1 < span.n) {  // S of the next step replaces P of the last
-          ok = wait(sm.k_full, i + 1) && (i == 0 || wait(sm.o_full, i - 1));
+      for (uint32_t i = 0; i < min(2u, steps) && ok; i++) {
+        ok = wait(sm.k_full, i);
+        if (ok) scores(i);
+      }
+      for (uint32_t i = 0; i < steps && ok; i++) {
+        // the scores of step i + 2 replace the weights of step i - 1 (what follows is issued by this thread)
+        ok = i == 0 || wait(sm.o_full, i - 1);
+        if (i + 2 < steps) {
+          ok = ok && wait(sm.k_full, i + 2);  // next: keys of i + 4, after S of i + 2
           tc_fence_after();
-          if (ok) scores(i + 1);
+          if (ok) scores(i + 2);
         }
-        ok = ok && wait(sm.v_full, i) && wait(sm.p_full, i) && (i < 2 || wait(sm.o_free, i - 2));
+        // next: values of i + 2, after O of i; weights of i + 3, after its S; O of step i read, after it is made
+        ok = ok && wait(sm.v_full, i) && wait(sm.p_full, i) && (i == 0 || wait(sm.o_free, i - 1));
         tc_fence_after();
         if (!ok) break;
-#pragma unroll
+#pragma unroll 1
         for (uint32_t part = 0; part < 2; part++)
 #pragma unroll
-          for (uint32_t ks = 0; ks < KQ_PAGE / 16; ks++)
-            kr_mma_ts(tm + KR_O + (i & 1) * HD, tm + KR_S + (i & 1) * KQ_PAGE + part * 32 + ks * 8,
+          for (uint32_t ks = 0; ks < KR_POS / 16; ks++)
+            kr_mma_ts(tm + KR_O, tm + KR_S + i % KR_NS * KR_POS + ks / 2 * 32 + (part ? 0 : 16) + ks % 2 * 8,
                       umma_desc(sm.v[i & 1] + ks * 2 * (HD / 8) * 64, (HD / 8) * 128, 128), kr_idesc<HD>(),
                       part || ks);
-        umma_commit(&sm.o_full[i & 1]);
+        umma_commit(&sm.o_full);
       }
       umma_commit(&sm.fin);  // everything issued, whether or not a wait ran out
       mbar_wait(&sm.fin, 0);
     }
     __syncwarp();
-  } else if (warp >= 8) {
-    const uint32_t cw = warp - 8, g = lane & 7;
-    // 512-byte tiles of a page's side, taken in turn by the warps: 8 KJ of keys,
-    // 4 KJ pairs of values
-    constexpr uint32_t NK = 8 * KJ, NP = 4 * KJ, KX = (NK + KR_CONV - 1) / KR_CONV, VX = (NP + KR_CONV - 1) / KR_CONV;
-    uint4 kr[KX], vr[2 * VX];
-    // the lane's pieces: keys of position g of the tile's 8, dims 16 t .. (t =
-    // lane / 8); values of pieces t = 2 tp, 2 tp + 1 (tp = lane / 8 % 2) of the
-    // pair's tile lane / 16
-    auto load_k = [&](uint32_t page) {
-      const uint8_t* src = a.c.codes + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_PAGE * HD + g * 64 + (lane >> 3) * 16;
+  } else if (warp >= 12) {
+    const uint32_t cw = warp - 12, g = lane & 7;
+    // a page's keys are 8 KJ tiles of 8 positions x 64 dims; the lane takes dims 16 (lane / 8) .. of position lane % 8.
+    // A step's tiles are taken in turn by the warps, and loaded a step ahead.
+    constexpr uint32_t NT = 16 * KJ, X = (NT + KR_CONV - 1) / KR_CONV;
+    uint4 w[X];
+    auto load = [&](uint32_t pa, uint32_t pb) {
+      const uint8_t* src = a.c.codes + (uint64_t)kvh * 2 * KQ_PAGE * HD + g * 64 + (lane >> 3) * 16;
+      const uint64_t stride = (uint64_t)a.c.nkv * 2 * KQ_PAGE * HD;
 #pragma unroll
-      for (uint32_t x = 0; x < KX; x++)
-        if (cw + KR_CONV * x < NK) kr[x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 512));
+      for (uint32_t x = 0; x < X; x++) {
+        const uint32_t tile = cw + KR_CONV * x;
+        if (tile < NT)
+          w[x] = __ldg(reinterpret_cast<const uint4*>(src + (tile < NT / 2 ? pa : pb) * stride + tile % (NT / 2) * 512));
+      }
     };
-    auto load_v = [&](uint32_t page) {
-      const uint8_t* src = a.c.codes + (((uint64_t)page * a.c.nkv + kvh) * 2 + 1) * KQ_PAGE * HD + g * 64 +
-                           (lane >> 4) * 512 + (lane >> 3 & 1) * 32;
+    KrPages ids(page_of, lane);
+    load(ids.at(0), ids.at(1));
+    for (uint32_t i = 0; i < steps; i++) {
+      ids.move(page_of, lane, 2 * i + 2);
+      const uint32_t pa = ids.at(2 * i + 2), pb = ids.at(2 * i + 3);
+      // S of step i - 2 has read the keys; next: S of i + 1, after its keys
+      ok = __all_sync(0xffffffffu, i < 2 || wait(sm.s_full, i - 2));
+      if (!ok) break;
+      __half* dst = sm.k[i & 1] + g * 8;
 #pragma unroll
-      for (uint32_t x = 0; x < VX; x++)
-        if (cw + KR_CONV * x < NP) {
-          vr[2 * x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 1024));
-          vr[2 * x + 1] = __ldg(reinterpret_cast<const uint4*>(src + (cw + KR_CONV * x) * 1024 + 16));
-        }
-    };
-    auto put_k = [&](__half* dst) {
-#pragma unroll
-      for (uint32_t x = 0; x < KX; x++) {
-        const uint32_t tile = cw + KR_CONV * x, tg = tile / KJ, kc = (tile % KJ * 4 + (lane >> 3)) * 2;
-        if (tile >= NK) continue;
+      for (uint32_t x = 0; x < X; x++) {
+        const uint32_t tile = cw + KR_CONV * x, kc = (tile % KJ * 4 + (lane >> 3)) * 2;
+        if (tile >= NT) continue;
         uint32_t h[8];
-        kq_halves(kr[x].x, h);
-        kq_halves(kr[x].y, h + 2);
-        kq_halves(kr[x].z, h + 4);
-        kq_halves(kr[x].w, h + 6);
-        __half* at = dst + (kc * (KQ_PAGE / 8) + tg) * 64 + g * 8;
+        kq_halves(w[x].x, h);
+        kq_halves(w[x].y, h + 2);
+        kq_halves(w[x].z, h + 4);
+        kq_halves(w[x].w, h + 6);
+        __half* at = dst + (kc * (KR_POS / 8) + tile / KJ) * 64;
         *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(at + (KQ_PAGE / 8) * 64) = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(at + (KR_POS / 8) * 64) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-    };
-    auto put_v = [&](__half* dst) {
-#pragma unroll
-      for (uint32_t x = 0; x < VX; x++) {
-        if (cw + KR_CONV * x >= NP) continue;
-        const uint32_t tile = 2 * (cw + KR_CONV * x) + (lane >> 4), blk = tile / (HD / 32), q = tile % (HD / 32);
-        const uint32_t kc = blk * 2 + (lane >> 3 & 1);
-        const uint32_t wa[4] = {vr[2 * x].x, vr[2 * x].y, vr[2 * x].z, vr[2 * x].w};
-        const uint32_t wb[4] = {vr[2 * x + 1].x, vr[2 * x + 1].y, vr[2 * x + 1].z, vr[2 * x + 1].w};
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-          uint32_t h[4];
-          kq_halves(wa[i], h);
-          kq_halves(wb[i], h + 2);
-          *reinterpret_cast<uint4*>(dst + (kc * (HD / 8) + q * 4 + i) * 64 + g * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-      }
-    };
-    auto full = [&](uint64_t* bar) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    uint32_t next = page_of(0);
-    load_k(next);
-    load_v(next);
-    next = page_of(1);
-    for (uint32_t i = 0; i < span.n; i++) {
-      ok = i < 2 || wait(sm.s_full, i - 2);  // S of step i - 2 has read the keys
-      if (!ok) break;
-      put_k(sm.k[i & 1]);
-      full(&sm.k_full[i & 1]);
-      load_k(next);
-      ok = i < 2 || wait(sm.o_full, i - 2);  // its O the values
-      if (!ok) break;
-      put_v(sm.v[i & 1]);
-      full(&sm.v_full[i & 1]);
-      load_v(next);
-      next = page_of(i + 2);
+      if (lane == 0) mbar_arrive(&sm.k_full[i & 1]);
+      load(pa, pb);
     }
-  } else if (warp >= 4) {
-    const uint32_t row = tid - 128, lanes = ((warp & 3) * 32) << 16;
+  } else if (warp >= 8) {
+    kr_regs_inc<KR_REG_ACC>();
+    const uint32_t row = tid & 127, lanes = ((warp & 3) * 32) << 16, cw = warp - 8, g = lane & 7;
+    // a page's values are 8 KJ tiles of 16 positions x 32 dims, taken in pairs; the lane takes pieces t = 2 tp, 2 tp + 1
+    // (tp = lane / 8 % 2) of dims 8 c + lane % 8 of the pair's tile lane / 16
+    constexpr uint32_t X = KJ;  // pairs of a page for one of four warps
+    uint4 w[2][2 * X];
+    auto load = [&](uint32_t page, uint4* v) {
+      const uint8_t* src = a.c.codes + (((uint64_t)page * a.c.nkv + kvh) * 2 + 1) * KQ_PAGE * HD + (lane >> 4) * 512 +
+                           g * 64 + (lane >> 3 & 1) * 32;
+#pragma unroll
+      for (uint32_t x = 0; x < X; x++) {
+        v[2 * x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024));
+        v[2 * x + 1] = __ldg(reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024 + 16));
+      }
+    };
+    KrPages ids(page_of, lane);
+    auto values = [&](uint32_t i) {  // the operand of step i; the codes of step i + 1 start to load
+#pragma unroll
+      for (uint32_t page = 0; page < 2; page++)
+#pragma unroll
+        for (uint32_t x = 0; x < X; x++) {
+          const uint32_t tile = 2 * (cw + 4 * x) + (lane >> 4), q = tile % (HD / 32);
+          const uint32_t kc = page * 8 + tile / (HD / 32) * 2 + (lane >> 3 & 1);
+          const uint4 va = w[page][2 * x], vb = w[page][2 * x + 1];
+          const uint32_t u[4] = {va.x, va.y, va.z, va.w}, z[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+          for (uint32_t c = 0; c < 4; c++) {
+            uint32_t h[4];
+            kq_halves(u[c], h);
+            kq_halves(z[c], h + 2);
+            *reinterpret_cast<uint4*>(sm.v[i & 1] + (kc * (HD / 8) + q * 4 + c) * 64 + g * 8) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.v_full[i & 1]);
+      ids.move(page_of, lane, 2 * i + 2);
+      load(ids.at(2 * i + 2), w[0]);
+      load(ids.at(2 * i + 3), w[1]);
+    };
+    load(ids.at(0), w[0]);
+    load(ids.at(1), w[1]);
+    values(0);
     float acc[HD];
 #pragma unroll
     for (int d = 0; d < HD; d++) acc[d] = 0.f;
-    for (uint32_t i = 0; i < span.n; i++) {
-      ok = __all_sync(0xffffffffu, wait(sm.p_full, i) && wait(sm.o_full, i));
+    for (uint32_t i = 0; i < steps; i++) {
+      if (i + 1 < steps) values(i + 1);  // O of step i - 1, the operand's last reader, is done: it has been added
+      // next: alpha of i + 4, after S of i + 4, after O of i + 1, after O of i has been read; O of i + 1, after that too
+      ok = __all_sync(0xffffffffu, wait(sm.a_full, i) && wait(sm.o_full, i));
       if (!ok) break;
       tc_fence_after();
-      const float alpha = sm.alpha[i & 1][row];
+      const float alpha = sm.alpha[i & 3][row];
 #pragma unroll
       for (int d = 0; d < HD; d += 16) {
         float o[16];
-        kr_ld16(tm + lanes + KR_O + (i & 1) * HD + d, o);
+        kr_ld16(tm + lanes + KR_O + d, o);
         kr_wait_ld(o);
 #pragma unroll
         for (int k = 0; k < 16; k++) acc[d + k] = fmaf(acc[d + k], alpha, o[k]);
       }
       tc_fence_before();
-      mbar_arrive(&sm.o_free[i & 1]);
+      mbar_arrive(&sm.o_free);
     }
     ok = ok && mbar_wait(&sm.l_full, 0);
     const uint32_t rr = r0 + row;
     if (ok && rr < nrows) {
-      const float l = sm.l[row], inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
+      // each warpgroup's denominator goes by the maximum of its own last step; the sums by that of the last
+      const float m0 = sm.last[0][row], m1 = sm.last[1][row], top = fmaxf(m0, m1);
+      const float l = (m0 == -INFINITY ? 0.f : sm.l[0][row] * kq_exp2(m0 - top)) +
+                      (m1 == -INFINITY ? 0.f : sm.l[1][row] * kq_exp2(m1 - top));
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
       T* out = a.out + (uint64_t)(s.row0 + rr / a.c.group) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD;
 #pragma unroll
       for (int d = 0; d < HD; d += 4) {
@@ -1184,69 +1258,103 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       }
     }
   } else {
-    const uint32_t row = tid, lanes = (warp * 32) << 16;
+    kr_regs_dec<KR_REG_OTHER>();
+    const uint32_t row = tid & 127, wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, side = lane >> 2 & 1;
     const float rowf = sm.rowf[row];
     const uint32_t rowpos = sm.rowpos[row];
-    KrRow r;
-    auto scales = [&](uint32_t page, float4* k4, float4* v4) {
-      const float4* p = reinterpret_cast<const float4*>(a.c.scales + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_NB);
-      *k4 = __ldg(p);
-      *v4 = __ldg(p + 1);
+    float m = -INFINITY, l = 0.f;
+    // a step's scales, one block a lane (lanes 0-7 and their likes), loaded two steps ahead
+    auto scales = [&](uint32_t page, float* ks, float* vs) {
+      const float* p = a.c.scales + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_NB + (lane & 3);
+      *ks = __ldg(p);
+      *vs = __ldg(p + KQ_NB);
     };
-    float4 k4, v4;
-    scales(page_of(0), &k4, &v4);
-    uint32_t next = page_of(1);
-    for (uint32_t i = 0; i < span.n; i++) {
-      const float f[4] = {k4.x * rowf, k4.y * rowf, k4.z * rowf, k4.w * rowf}, v[4] = {v4.x, v4.y, v4.z, v4.w};
-      scales(next, &k4, &v4);
-      next = page_of(i + 2);
-      ok = __all_sync(0xffffffffu, wait(sm.s_full, i));
+    float ks_next, vs_next;
+    scales(page_of(2 * wg + side), &ks_next, &vs_next);
+    uint32_t next = page_of(2 * wg + 4 + side);
+    for (uint32_t i = wg; i < steps; i += 2) {
+      const float ks = ks_next, vs = vs_next, lv = __log2f(fmaxf(vs, KQ_MIN_SCALE));
+      scales(next, &ks_next, &vs_next);
+      next = page_of(2 * i + 8 + side);
+      ok = __all_sync(0xffffffffu, wait(sm.s_full, i));  // next: S of i + 3, after O of i, after this step's weights
       if (!ok) break;
       tc_fence_after();
-      const uint32_t t = tm + lanes + KR_S + (i & 1) * KQ_PAGE;
-      float x[64];
+      const uint32_t t = tm + lanes + KR_S + i % KR_NS * KR_POS;
+      const bool none = 2 * i + 1 >= span.n;  // the last step has one page
+      const uint32_t pos[2] = {span.page(2 * i) * KQ_PAGE, span.page(2 * i + 1) * KQ_PAGE};
+      bool masked = none;
 #pragma unroll
-      for (int b = 0; b < 4; b++) kr_ld16(t + 16 * b, x + 16 * b);
-#pragma unroll
-      for (int b = 0; b < 4; b++) kr_wait_ld(x + 16 * b);
-      const uint32_t pos = span.page(i) * KQ_PAGE;
-      const bool masked = pos + KQ_PAGE - 1 > plo || (a.window && pos + KQ_PAGE > a.sinks && phi - min(pos, phi) >= a.window);
-      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
-      float top;
-      if (masked) {
-#pragma unroll
-        for (uint32_t w = 0; w < 2; w++) {
-          const uint32_t base = pos + 32 * w, end = rowpos + 1, from = a.window && end > a.window ? end - a.window : 0;
-          vis[w] = kr_bits(base, from, end);
-          if (a.window) vis[w] |= kr_bits(base, 0, min(a.sinks, end));
+      for (int k = 0; k < 2; k++)
+        masked = masked || pos[k] + KQ_PAGE - 1 > plo ||
+                 (a.window && pos[k] + KQ_PAGE > a.sinks && phi - min(pos[k], phi) >= a.window);
+      // the positions 32 j .. of the step that the row sees
+      auto vis = [&](uint32_t j) {
+        const uint32_t base = (j < 2 ? pos[0] : pos[1]) + 32 * (j & 1), end = rowpos + 1;
+        uint32_t bits = kr_bits(base, a.window && end > a.window ? end - a.window : 0, end);
+        if (a.window) bits |= kr_bits(base, 0, min(a.sinks, end));
+        return none && j >= 2 ? 0u : bits;
+      };
+      float top = -INFINITY;
+#pragma unroll 1
+      for (uint32_t j = 0; j < 4; j++) {
+        const float f0 = __shfl_sync(0xffffffffu, ks, 2 * j) * rowf, f1 = __shfl_sync(0xffffffffu, ks, 2 * j + 1) * rowf;
+        const float a0 = __shfl_sync(0xffffffffu, lv, 2 * j), a1 = __shfl_sync(0xffffffffu, lv, 2 * j + 1);
+        float x[32];
+        kr_ld32(t + 32 * j, x);
+        kr_wait_ld(x);
+        kr_wait_ld(x + 16);
+        if (masked) {
+          const uint32_t bits = vis(j);
+          top = fmaxf(top, fmaxf(kr_top<true>(x, f0, a0, bits), kr_top<true>(x + 16, f1, a1, bits >> 16)));
+        } else {
+          top = fmaxf(top, fmaxf(kr_top<false>(x, f0, a0, 0), kr_top<false>(x + 16, f1, a1, 0)));
         }
-        top = kr_top<true>(x, f, v, vis);
-      } else {
-        top = kr_top<false>(x, f, v, vis);
       }
-      const float mn = fmaxf(r.m, top), c = mn == r.m ? 1.f : kq_exp2(r.m - mn);
-      r.m = mn;
-      r.l *= c;
-      if (masked)
-        kr_weights<true>(x, f, v, vis, r, t);
-      else
-        kr_weights<false>(x, f, v, vis, r, t);
+      float before = -INFINITY;
+      if (i) {  // next: the maximum of i + 1, after this step's
+        ok = __all_sync(0xffffffffu, wait(sm.m_full, i - 1));
+        if (!ok) break;
+        before = sm.m[(i - 1) & 1][row];
+      }
+      const float mn = fmaxf(before, top), sub = mn == -INFINITY ? 0.f : mn;
+      sm.m[i & 1][row] = mn;
+      mbar_arrive(&sm.m_full[i & 1]);
+      sm.alpha[i & 3][row] = mn == before ? 1.f : kq_exp2(before - mn);  // step i - 4's has been read: O of i - 3 is made
+      mbar_arrive(&sm.a_full[i & 3]);
+      l = mn == m ? l : l * kq_exp2(m - mn);
+      m = mn;
+#pragma unroll 1
+      for (uint32_t j = 0; j < 4; j++) {
+        const float f0 = __shfl_sync(0xffffffffu, ks, 2 * j) * rowf, f1 = __shfl_sync(0xffffffffu, ks, 2 * j + 1) * rowf;
+        const float v0 = __shfl_sync(0xffffffffu, vs, 2 * j), v1 = __shfl_sync(0xffffffffu, vs, 2 * j + 1);
+        const float a0 = __shfl_sync(0xffffffffu, lv, 2 * j), a1 = __shfl_sync(0xffffffffu, lv, 2 * j + 1);
+        float x[32];
+        kr_ld32(t + 32 * j, x);
+        kr_wait_ld(x);
+        kr_wait_ld(x + 16);
+        if (!masked && fminf(v0, v1) >= KQ_MIN_SCALE) {
+          const float lp = 13.f - sub;  // log2 KR_P - m
+          l = fmaf(kr_weights(x, f0, a0 + lp), __fdividef(1.f / KR_P, v0), l);
+          l = fmaf(kr_weights(x + 16, f1, a1 + lp), __fdividef(1.f / KR_P, v1), l);
+        } else {
+          const uint32_t bits = masked ? vis(j) : 0xffffffffu;
+          l += kr_weights_masked(x, f0, v0 * KR_P, sub, bits) + kr_weights_masked(x + 16, f1, v1 * KR_P, sub, bits >> 16);
+        }
+        kr_put(x, t + 32 * j);
+        kr_put(x + 16, t + 32 * j + 8);
+      }
       kr_wait_st();
-      ok = i < 2 || wait(sm.o_free, i - 2);  // alpha of step i - 2 has been read
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      sm.alpha[i & 1][row] = c;
       tc_fence_before();
-      mbar_arrive(&sm.p_full[i & 1]);
+      mbar_arrive(&sm.p_full[i % KR_NS]);
     }
-    sm.l[row] = r.l;
+    sm.l[wg][row] = l;
+    sm.last[wg][row] = m;
     mbar_arrive(&sm.l_full);
   }
   if (!ok && lane == 0) atomicOr(a.c.status, KQ_TIMEOUT);
   tc_fence_before();
   __syncthreads();
-  if (warp == 11)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kr_tmem<HD>) : "memory");
+  if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
 }
 
 // ---------------------------------------------------------------------------
