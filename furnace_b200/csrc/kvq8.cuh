@@ -17,13 +17,10 @@ constexpr uint32_t KQ_PAGE = 64;   // positions of a page
 constexpr uint32_t KQ_BLOCK = 16;  // positions that share a scale
 constexpr uint32_t KQ_NB = KQ_PAGE / KQ_BLOCK;
 
-// Byte offset inside a block of key (tok, dim) and value (tok, dim).
+// Byte offset inside a block of key (tok, dim).
 template <int HD>
 __device__ __forceinline__ uint32_t kq_koff(uint32_t tok, uint32_t dim) {
   return (tok >> 3) * 8 * HD + (dim >> 6) * 512 + (tok & 7) * 64 + (dim & 63);
-}
-__device__ __forceinline__ uint32_t kq_voff(uint32_t tok, uint32_t dim) {
-  return (dim >> 5) * 512 + (dim & 7) * 64 + ((tok & 7) >> 1) * 16 + ((dim & 31) >> 3) * 4 + (tok >> 3) * 2 + (tok & 1);
 }
 
 struct KqSeq {
@@ -51,15 +48,21 @@ __device__ __forceinline__ KqSeq kq_seq(const KvQ8Batch& b, uint32_t i, uint32_t
   return s;
 }
 
-// Physical page of sequence i's page j, or -1 (status) when it is none.
-__device__ __forceinline__ int32_t kq_page(const KvQ8Dev& c, const KvQ8Batch& b, uint32_t i, uint32_t j) {
+// Physical page of sequence i's page j as the table has it, and checked: -1
+// (status) when it is none.
+__device__ __forceinline__ int64_t kq_entry(const KvQ8Batch& b, uint32_t i, uint32_t j) {
   const int64_t at = (int64_t)i * b.max_pages + j;
-  const int64_t p = b.pages ? (int64_t)b.pages[at] : at;
+  return b.pages ? (int64_t)b.pages[at] : at;
+}
+__device__ __forceinline__ int32_t kq_checked(const KvQ8Dev& c, int64_t p) {
   if (p < 0 || p >= c.n_pages) {
     atomicOr(c.status, KQ_BAD_PAGE);
     return -1;
   }
   return (int32_t)p;
+}
+__device__ __forceinline__ int32_t kq_page(const KvQ8Dev& c, const KvQ8Batch& b, uint32_t i, uint32_t j) {
+  return kq_checked(c, kq_entry(b, i, j));
 }
 
 __device__ __forceinline__ float kq_ld(const float* p) { return *p; }
@@ -67,37 +70,238 @@ __device__ __forceinline__ float kq_ld(const __half* p) { return __half2float(*p
 __device__ __forceinline__ void kq_st(float* p, float v) { *p = v; }
 __device__ __forceinline__ void kq_st(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Element d of a head's row, rotated at a position's factors cs (null: as it
-// is): pairs half a head apart, every product rounded by itself (the
-// reference's uncontracted a*c - b*s / a*s + b*c, src/model.rs:193-217).
-template <int HD, typename T>
-__device__ __forceinline__ float kq_rotated(const T* x, const float2* cs, uint32_t d) {
-  constexpr uint32_t half = HD / 2;
-  const float own = kq_ld(x + d);
-  if (!cs) return own;
-  const float2 f = cs[d % half];
-  const float other = kq_ld(x + (d < half ? d + half : d - half));
-  return d < half ? __fsub_rn(__fmul_rn(own, f.x), __fmul_rn(other, f.y))
-                  : __fadd_rn(__fmul_rn(other, f.y), __fmul_rn(own, f.x));
+// code + 128 of x at scale s (code 0 for an empty scale): round(x / s).
+__device__ __forceinline__ uint32_t kq_code(float x, float s) {
+  return 128 + (s > 0.f ? __float2int_rn(fminf(fmaxf(__fdiv_rn(x, s), -127.f), 127.f)) : 0);
+}
+// The same for n values, in the low bytes of w.  The product with inv = 1 / s,
+// rounded to an integer by adding 1.5 * 2^23 in one operation, is off by at most
+// 1.6e-5 before the rounding for a code up to 127, so the division, several
+// times the work, is left to threads with a value near a border (and to scales
+// too small for an inverse).
+template <int N>
+__device__ __forceinline__ void kq_codes(const float* x, float s, float inv, uint32_t* w) {
+  constexpr float magic = 12582912.f + 128.f;
+  bool near = !(s > 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float y = __fmaf_rn(x[i], inv, magic), q = __fsub_rn(y, magic);
+    near |= !(fabsf(__fmaf_rn(x[i], inv, -q)) <= 0.49998f);
+    w[i] = __float_as_uint(y);
+  }
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = kq_code(x[i], s);
+  }
+}
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t kq_bytes(const uint32_t* w) {
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+}
+// code + 128 of an older byte under a scale that grew by 1 / ratio
+__device__ __forceinline__ uint32_t kq_recode(uint32_t byte, float ratio) {
+  return 128 + __float2int_rn(__fmul_rn((float)((int)byte - 128), ratio));
 }
 
-// code of x at scale s (0 for an empty scale)
-__device__ __forceinline__ int kq_code(float x, float s) {
-  return s > 0.f ? __float2int_rn(fminf(fmaxf(__fdiv_rn(x, s), -127.f), 127.f)) : 0;
+// N consecutive, aligned elements at p.
+template <int N>
+__device__ __forceinline__ void kq_ldn(const float* p, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if constexpr (N >= 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(p);
+      x[0] = v.x, x[1] = v.y;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void kq_ldn(const __half* p, float* x) {
+  uint32_t w[N / 2];
+  if constexpr (N >= 8) {
+#pragma unroll
+    for (int i = 0; i < N / 8; i++) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 8 * i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+#pragma unroll
+  for (int i = 0; i < N / 2; i++) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Append.  Grid (blocks a sequence can touch, nkv, n_seqs): a CTA quantizes
-// one block of one head, keys and values.  The scale is the largest magnitude
-// of the call's values / 127, and at least the block's older scale when
-// positions before this call's are kept; those take the codes of the larger
-// scale.  Every position of the block is one step of a plain loop here.
+// one block of one head, its first half keys, its second half values; a thread
+// takes two 16-byte pieces, so that the call's values are read once and every
+// store is a whole piece.  A key thread's pieces are the two halves of its
+// rotated pairs.  Scale: the largest magnitude of the call's values / 127, and
+// at least the block's older scale when positions before this call's are kept;
+// those take the codes of the larger scale.  Bound by the bytes of k and v: the
+// loads of a thread are all under way before the first is used.
 // ---------------------------------------------------------------------------
-constexpr int KQ_AP_THREADS = 128;
+template <int HD, typename T>
+__global__ void __launch_bounds__(HD) k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k,
+                                                    const T* __restrict__ v, uint64_t ld) {
+  pdl_trigger();
+  pdl_wait();
+  const KqSeq s = kq_seq(b, blockIdx.z, c.status);
+  const int32_t p0 = s.len - s.n_new;
+  const int32_t blk = p0 / (int32_t)KQ_BLOCK + (int32_t)blockIdx.x, base = blk * (int32_t)KQ_BLOCK;
+  if (s.n_new == 0 || base >= s.len) return;
+  if (c.rope && s.len > (int64_t)c.n_rope) {
+    if (threadIdx.x == 0) atomicOr(c.status, KQ_BAD_POS);
+    return;
+  }
+  const int64_t entry = kq_entry(b, blockIdx.z, blk / KQ_NB);  // looked at once the values are on their way
+  constexpr uint32_t U = HD / 2, half = HD / 2;  // threads of a side
+  const uint32_t h = blockIdx.y, side = threadIdx.x / U, u = threadIdx.x % U;
+  const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);  // new positions [a, e)
+  // this head's element (position base, 0)
+  const uint64_t first = (uint64_t)(s.row0 + base - p0) * ld + (uint64_t)h * HD;
+  // keys: position tok, dims d .. d + 15 and half + d ..; values: positions tok[k] = 2t, 2t + 1, 8 + 2t, 9 + 2t of dims
+  // 32 q + 8 i + g and HD / 2 + that
+  const uint32_t tok = u / (HD / 32), d = u % (HD / 32) * 16, g = u >> 2 & 7, t = u & 3, q = u >> 5;
+  float x[32];
+#pragma unroll
+  for (int i = 0; i < 32; i++) x[i] = 0.f;
+  if (side == 0) {
+    if ((int32_t)tok >= a && (int32_t)tok < e) {
+      const T* p = k + first + (uint64_t)tok * ld + d;
+      kq_ldn<16>(p, x);
+      kq_ldn<16>(p + half, x + 16);
+      if (c.rope) {
+        float f[32];
+        kq_ldn<32>(reinterpret_cast<const float*>(c.rope + (uint64_t)(base + tok) * half + d), f);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float m = x[i], w = x[16 + i];
+          x[i] = __fsub_rn(__fmul_rn(m, f[2 * i]), __fmul_rn(w, f[2 * i + 1]));
+          x[16 + i] = __fadd_rn(__fmul_rn(m, f[2 * i + 1]), __fmul_rn(w, f[2 * i]));
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int32_t y = (j >> 1) * 8 + 2 * t + (j & 1);
+      if (y >= a && y < e) {
+        const T* p = v + first + (uint64_t)y * ld + 32 * q + g;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[4 * i + j] = kq_ld(p + (i >> 2) * half + (i & 3) * 8);
+      }
+    }
+  }
+  const int32_t page = kq_checked(c, entry);
+  if (page < 0) return;
+  const uint64_t at = ((uint64_t)page * c.nkv + h) * 2 + side;
+  uint8_t* codes = c.codes + at * KQ_PAGE * HD + blk % KQ_NB * KQ_BLOCK * HD;
+  float* sc = c.scales + at * KQ_NB + blk % KQ_NB;
+  const float before = a > 0 ? *sc : 0.f;
+  uint4 kept[2];  // value pieces that hold older positions
+  if (side && a > 0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      kept[i] = *reinterpret_cast<const uint4*>(codes + (q + i * (HD / 64)) * 512 + g * 64 + t * 16);
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[i])));
+  if (!(top <= 3.402823466e38f)) {
+    atomicOr(c.status, KQ_NOT_FINITE);
+    top = INFINITY;
+  }
+  // largest magnitude of the side; non-negative floats order like their bits, and a side with a value that is not
+  // finite ends with infinity
+  __shared__ uint32_t s_top[2];
+  if (threadIdx.x < 2) s_top[threadIdx.x] = 0;
+  __syncthreads();
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0) atomicMax(&s_top[side], bits);
+  __syncthreads();
+  top = __uint_as_float(s_top[side]);
+  float scale = __fdiv_rn(top, 127.f);
+  if (a > 0 && !(scale > before)) scale = before;
+  if (top == INFINITY) scale = __int_as_float(0x7fffffff);  // no number, not a wrong one
+  const bool grew = a > 0 && scale > before;
+  const float ratio = __fdiv_rn(before, scale), inv = __fdiv_rn(1.f, scale);
+  if (u == 0) *sc = scale;
+  if (side == 0) {
+    uint4* dst[2] = {reinterpret_cast<uint4*>(codes + kq_koff<HD>(tok, d)),
+                     reinterpret_cast<uint4*>(codes + kq_koff<HD>(tok, half + d))};
+    if ((int32_t)tok >= e || ((int32_t)tok < a && !grew)) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      uint32_t w[4];
+      if ((int32_t)tok < a) {
+        const uint4 old = *dst[i];
+        const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+          w[m] = 0;
+#pragma unroll
+          for (int n = 0; n < 4; n++) w[m] |= kq_recode(o[m] >> (8 * n) & 255, ratio) << (8 * n);
+        }
+      } else {
+        uint32_t y[16];
+        kq_codes<16>(x + 16 * i, scale, inv, y);
+#pragma unroll
+        for (int m = 0; m < 4; m++) w[m] = kq_bytes(y + 4 * m);
+      }
+      *dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      uint4* dst = reinterpret_cast<uint4*>(codes + (q + i * (HD / 64)) * 512 + g * 64 + t * 16);
+      uint32_t w[4], y[16];
+      kq_codes<16>(x + 16 * i, scale, inv, y);
+#pragma unroll
+      for (int m = 0; m < 4; m++) w[m] = kq_bytes(y + 4 * m);
+      if (a > 0) {  // positions before the call's are kept
+        const uint32_t o[4] = {kept[i].x, kept[i].y, kept[i].z, kept[i].w};
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            if ((n >> 1) * 8 + 2 * (int32_t)t + (n & 1) >= a) continue;
+            const uint32_t byte = o[m] >> (8 * n) & 255;
+            w[m] = (w[m] & ~(255u << (8 * n))) | (grew ? kq_recode(byte, ratio) : byte) << (8 * n);
+          }
+      }
+      *dst = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Read-back: the rows a batch names as values.  Grid as for the append, a
+// block of one head a CTA; the pieces pass through shared memory, since a value
+// piece holds four positions of four dims.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void kq_st4(float* p, const float* x) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint32_t kq_pack(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void kq_st4(__half* p, const float* x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(kq_pack(x[0], x[1]), kq_pack(x[2], x[3]));
+}
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(KQ_AP_THREADS) k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k,
-                                                               const T* __restrict__ v, uint64_t ld) {
+__global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __restrict__ k, T* __restrict__ v,
+                                                  uint64_t ld) {
   pdl_trigger();
   pdl_wait();
   const KqSeq s = kq_seq(b, blockIdx.z, c.status);
@@ -106,80 +310,33 @@ __global__ void __launch_bounds__(KQ_AP_THREADS) k_kvq8_append(KvQ8Dev c, KvQ8Ba
   if (s.n_new == 0 || base >= s.len) return;
   const int32_t page = kq_page(c, b, blockIdx.z, blk / KQ_NB);
   if (page < 0) return;
-  if (c.rope && s.len > (int32_t)c.n_rope) {
-    if (threadIdx.x == 0) atomicOr(c.status, KQ_BAD_POS);
-    return;
-  }
-  const uint32_t h = blockIdx.y, tid = threadIdx.x, sub = blk % KQ_NB;
-  const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);  // new positions [a, e)
-  __shared__ float red[KQ_AP_THREADS / 32];
-  for (int w = 0; w < 2; w++) {
-    uint8_t* codes = c.codes + (((uint64_t)page * c.nkv + h) * 2 + w) * KQ_PAGE * HD + sub * KQ_BLOCK * HD;
-    float* sc = c.scales + (((uint64_t)page * c.nkv + h) * 2 + w) * KQ_NB + sub;
-    auto value = [&](int32_t tok, uint32_t d) {
-      const uint64_t at = (uint64_t)(s.row0 + base + tok - p0) * ld + (uint64_t)h * HD;
-      return w ? kq_ld(v + at + d)
-               : kq_rotated<HD>(k + at, c.rope ? c.rope + (uint64_t)(base + tok) * (HD / 2) : nullptr, d);
-    };
-    float m = 0.f;
-    bool bad = false;
-    for (int32_t tok = a; tok < e; tok++)
-      for (uint32_t d = tid; d < HD; d += KQ_AP_THREADS) {
-        const float x = fabsf(value(tok, d));
-        bad |= !(x <= 3.402823466e38f);
-        m = fmaxf(m, x);
-      }
-    if (bad) atomicOr(c.status, KQ_NOT_FINITE);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (__syncthreads_or(bad)) m = __int_as_float(0x7fffffff);  // a scale that is no number, not a wrong one
-    if (tid % 32 == 0) red[tid / 32] = m;
-    const float before = *sc;
-    __syncthreads();
-    bool nan = false;
-    for (int i = 0; i < KQ_AP_THREADS / 32; i++) {
-      nan |= red[i] != red[i];
-      m = fmaxf(m, red[i]);
-    }
-    float scale = __fdiv_rn(m, 127.f);
-    if (a > 0 && !(scale > before)) scale = before;
-    if (nan) scale = __int_as_float(0x7fffffff);
-    const bool grew = a > 0 && scale > before;
-    const float ratio = __fdiv_rn(before, scale);
-    for (int32_t tok = 0; tok < e; tok++)
-      for (uint32_t d = tid; d < HD; d += KQ_AP_THREADS) {
-        uint8_t* p = codes + (w ? kq_voff(tok, d) : kq_koff<HD>(tok, d));
-        if (tok >= a)
-          *p = (uint8_t)(128 + kq_code(value(tok, d), scale));
-        else if (grew)
-          *p = (uint8_t)(128 + __float2int_rn(__fmul_rn((float)((int)*p - 128), ratio)));
-      }
-    __syncthreads();  // every thread has read *sc and red
-    if (tid == 0) *sc = scale;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Read-back: the rows a batch names as values.  Grid (max_new, nkv, n_seqs).
-// ---------------------------------------------------------------------------
-template <int HD, typename T>
-__global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __restrict__ k, T* __restrict__ v,
-                                                  uint64_t ld) {
-  pdl_trigger();
-  pdl_wait();
-  const KqSeq s = kq_seq(b, blockIdx.z, c.status);
-  const uint32_t h = blockIdx.y, d = threadIdx.x;
-  if ((int32_t)blockIdx.x >= s.n_new) return;
-  const uint32_t pos = s.len - s.n_new + blockIdx.x;
-  const int32_t page = kq_page(c, b, blockIdx.z, pos / KQ_PAGE);
-  if (page < 0) return;
-  const uint32_t sub = pos / KQ_BLOCK % KQ_NB, tok = pos % KQ_BLOCK;
-  for (int w = 0; w < 2; w++) {
-    T* out = w ? v : k;
-    if (!out) continue;
-    const uint64_t side = ((uint64_t)page * c.nkv + h) * 2 + w;
-    const uint8_t code = c.codes[side * KQ_PAGE * HD + sub * KQ_BLOCK * HD + (w ? kq_voff(tok, d) : kq_koff<HD>(tok, d))];
-    kq_st(out + (uint64_t)(s.row0 + blockIdx.x) * ld + (uint64_t)h * HD + d,
-          __fmul_rn((float)((int)code - 128), c.scales[side * KQ_NB + sub]));
+  const uint32_t h = blockIdx.y, u = threadIdx.x;
+  const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);
+  __shared__ __align__(16) uint8_t tile[2][KQ_BLOCK][HD + 16];
+  const uint64_t at = ((uint64_t)page * c.nkv + h) * 2;
+  const uint8_t* codes = c.codes + at * KQ_PAGE * HD + blk % KQ_NB * KQ_BLOCK * HD;
+  const uint4 kp = *reinterpret_cast<const uint4*>(codes + u * 16);
+  const uint4 vp = *reinterpret_cast<const uint4*>(codes + KQ_PAGE * HD + u * 16);
+  const float sc[2] = {c.scales[at * KQ_NB + blk % KQ_NB], c.scales[(at + 1) * KQ_NB + blk % KQ_NB]};
+  const uint32_t g = u >> 2 & 7, t = u & 3, r = u >> 5;  // piece (g, t) of tile r
+  *reinterpret_cast<uint4*>(&tile[0][r / (HD / 64) * 8 + g][r % (HD / 64) * 64 + t * 16]) = kp;
+  const uint32_t w[4] = {vp.x, vp.y, vp.z, vp.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int n = 0; n < 4; n++) tile[1][(n >> 1) * 8 + 2 * t + (n & 1)][r * 32 + 8 * i + g] = (uint8_t)(w[i] >> (8 * n));
+  __syncthreads();
+  // four dims a thread
+#pragma unroll
+  for (uint32_t x = u; x < 2 * KQ_BLOCK * HD / 4; x += HD) {
+    const uint32_t side = x / (KQ_BLOCK * HD / 4), tok = x / (HD / 4) % KQ_BLOCK, d = x % (HD / 4) * 4;
+    T* out = side ? v : k;
+    if (!out || (int32_t)tok < a || (int32_t)tok >= e) continue;
+    const uint32_t bytes = *reinterpret_cast<const uint32_t*>(&tile[side][tok][d]);
+    float y[4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) y[n] = __fmul_rn((float)((int)(bytes >> (8 * n) & 255) - 128), sc[side]);
+    kq_st4(out + (uint64_t)(s.row0 + base + (int32_t)tok - p0) * ld + (uint64_t)h * HD + d, y);
   }
 }
 
@@ -294,10 +451,6 @@ __device__ __forceinline__ void kq_halves(uint32_t w, uint32_t* h) {
   h[0] = *reinterpret_cast<const uint32_t*>(&x);
   h[1] = *reinterpret_cast<const uint32_t*>(&y);
 }
-__device__ __forceinline__ uint32_t kq_pack(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // High and low parts of two values: hi = rn(x), lo = rn((x - hi) * 2^11).
 __device__ __forceinline__ void kq_split2(float a, float b, uint32_t* hi, uint32_t* lo) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -341,39 +494,6 @@ struct KqSplitArgs {
   uint64_t* prefix;     // [n_seqs + 1] cost before each sequence (written by CTA 0)
   float* slots;         // [2 * gridDim.x]
 };
-
-// A row's elements d .. d + N - 1 (N consecutive, aligned).
-template <int N>
-__device__ __forceinline__ void kq_ldn(const float* p, float* x) {
-  if constexpr (N == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else {
-    const float2 v = *reinterpret_cast<const float2*>(p);
-    x[0] = v.x, x[1] = v.y;
-  }
-}
-template <int N>
-__device__ __forceinline__ void kq_ldn(const __half* p, float* x) {
-  uint32_t w[N / 2];
-  if constexpr (N == 4) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-#pragma unroll
-  for (int i = 0; i < N / 2; i++) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void kq_st4(float* p, const float* x) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-__device__ __forceinline__ void kq_st4(__half* p, const float* x) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(kq_pack(x[0], x[1]), kq_pack(x[2], x[3]));
-}
 
 // Rows of one segment: 16 threads a row, each N pairs.  get() starts the
 // loads; put() rotates, scales the row by a power of two to a largest
@@ -723,8 +843,8 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_whole(const __grid_constant__ KqSplitArgs<HD, T> a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
-  pdl_wait();
   pdl_trigger();
+  pdl_wait();
   const KqPlan p = kq_plan(a.c, a.b, blockIdx.y, a.window, a.sinks);
   const uint32_t kvh = blockIdx.x % a.c.nkv, grp = blockIdx.x / a.c.nkv;
   if (grp < p.groups) kq_segment<HD, T>(a, sm, p, blockIdx.y, kvh, grp, 0, p.span.n, nullptr);
@@ -990,8 +1110,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   KrSmem<HD>& sm = *reinterpret_cast<KrSmem<HD>*>(smem_raw);
   constexpr uint32_t half = HD / 2, KJ = HD / 64;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, seq = blockIdx.z;
-  pdl_wait();
   pdl_trigger();
+  pdl_wait();
   const KqSeq s = kq_plan(a.c, a.b, seq, 0, 0).s;
   const uint32_t nrows = (uint32_t)s.n_new * a.c.group, tiles = (nrows + KR_M - 1) / KR_M;
   if (blockIdx.x >= tiles) return;
@@ -1360,11 +1480,14 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
+// Blocks that max_new consecutive positions can touch.
+static uint32_t kvq8_blocks(const KvQ8Batch& b) { return (b.max_new + 2 * KQ_BLOCK - 2) / KQ_BLOCK; }
+
 template <int HD, typename T>
 static void kvq8_append_t(const KvQ8Dev& c, const KvQ8Batch& b, const void* k, const void* v, uint64_t ld,
                           cudaStream_t s) {
-  const dim3 grid((b.max_new + 2 * KQ_BLOCK - 2) / KQ_BLOCK, c.nkv, b.n_seqs);
-  launch_pdl(k_kvq8_append<HD, T>, grid, dim3(KQ_AP_THREADS), 0, s, c, b, static_cast<const T*>(k),
+  const dim3 grid(kvq8_blocks(b), c.nkv, b.n_seqs);
+  launch_pdl(k_kvq8_append<HD, T>, grid, dim3(HD), 0, s, c, b, static_cast<const T*>(k),
              static_cast<const T*>(v), ld);
 }
 
@@ -1379,7 +1502,7 @@ void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const vo
 
 template <int HD, typename T>
 static void kvq8_read_t(const KvQ8Dev& c, const KvQ8Batch& b, void* k, void* v, uint64_t ld, cudaStream_t s) {
-  launch_pdl(k_kvq8_read<HD, T>, dim3(b.max_new, c.nkv, b.n_seqs), dim3(HD), 0, s, c, b, static_cast<T*>(k),
+  launch_pdl(k_kvq8_read<HD, T>, dim3(kvq8_blocks(b), c.nkv, b.n_seqs), dim3(HD), 0, s, c, b, static_cast<T*>(k),
              static_cast<T*>(v), ld);
 }
 
