@@ -33,7 +33,7 @@ BLOCK = {F32: (1, 4), F16: (1, 2), Q8_0: (32, 34), Q5_0: (32, 22), Q4_K: (256, 1
 TYPE_NAMES = {F32: "F32", F16: "F16", Q5_0: "Q5_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q6_K: "Q6_K"}
 
 FZ_OK, FZ_EINVAL, FZ_EFORMAT, FZ_EIO, FZ_ECUDA, FZ_ENOMEM, FZ_ETIMEOUT, FZ_ESPACE = range(8)
-FZ_KV_F32, FZ_KV_F16 = 0, 1  # KV cache element types
+FZ_KV_F32, FZ_KV_F16, FZ_KV_Q8 = 0, 1, 2  # KV cache element types
 
 # Every symbol include/furnace.h declares.
 EXPORTS = [
@@ -48,7 +48,7 @@ EXPORTS = [
     "fz_tokenizer_encode", "fz_tokenizer_decode", "fz_tokenizer_token_bytes", "fz_pretokenize", "fz_chat_template",
     "fz_utf8_stream_new", "fz_utf8_stream_free", "fz_utf8_stream_push", "fz_utf8_stream_flush",
     "fz_selftest_exchange_timeout", "fz_kvq8_append_dev", "fz_kvq8_attend_dev", "fz_kvq8_attend_work",
-    "fz_kvq8_read_dev", "fz_kvq8_status",
+    "fz_kvq8_read_dev", "fz_kvq8_status", "fz_kv_set_window",
 ]
 
 OPS = ["embed", "qkv", "rope_append", "attention", "o_proj", "gate_up", "down", "lm_head", "finalize"]
@@ -130,6 +130,7 @@ def load_library(build_if_missing: bool = True):
         "fz_kv_free": (None, [P]),
         "fz_kv_len": (I, [P, u32p]),
         "fz_kv_set_len": (I, [P, U32]),
+        "fz_kv_set_window": (I, [P, U32, U32]),
         "fz_kv_read": (I, [P, U32, I, U32, fp]),
         "fz_forward": (I, [P, P, u32p, U32, fp, u32p]),
         "fz_forward_last": (I, [P, u32p, U32, fp, u32p]),
@@ -421,8 +422,9 @@ class KvCache:
     """KvCache (src/model.rs:321-363), resident in HBM."""
 
     def __init__(self, model: Model, max_ctx: int, kv_dtype: int = 0):
-        """kv_dtype FZ_KV_F32 (the reference's f32 cache) or FZ_KV_F16
-        (binary16 elements, rounded to nearest even when appended)."""
+        """kv_dtype FZ_KV_F32 (the reference's f32 cache), FZ_KV_F16 (binary16
+        elements, rounded to nearest even when appended) or FZ_KV_Q8 (8-bit
+        codes, a scale per 16 positions, KV head and side)."""
         self.model = model
         self.max_ctx = max_ctx
         self.kv_dtype = kv_dtype
@@ -454,6 +456,11 @@ class KvCache:
     def reset(self):
         """len = 0: the cache reused for a new sequence."""
         _check(load_library().fz_kv_reset(self._h))
+
+    def set_window(self, window: int, sinks: int = 0):
+        """Attention over the last `window` positions (0: all) and the first
+        `sinks` only; FZ_KV_Q8 caches (fz_kv_set_window)."""
+        _check(load_library().fz_kv_set_window(self._h, window, sinks))
 
     def bytes(self) -> int:
         """KvCache::bytes (src/model.rs:341-343): K and V bytes of this rank."""
@@ -608,11 +615,13 @@ class Sampler:
 
 
 def generate_sampled(model: Model, prompt_ids, max_new: int, sampler: Sampler, stop_ids=(),
-                     max_ctx: int | None = None) -> np.ndarray:
+                     max_ctx: int | None = None, kv_dtype: int = 0, window: int = 0, sinks: int = 0) -> np.ndarray:
     """generate (src/generate.rs:83-157) with any sampler (fz_generate)."""
     p = np.ascontiguousarray(prompt_ids, dtype=np.uint32)
     max_ctx = max_ctx or min(model.config.context_length, 4096)
-    cache = KvCache(model, max_ctx)
+    cache = KvCache(model, max_ctx, kv_dtype)
+    if window or sinks:
+        cache.set_window(window, sinks)
     st = np.ascontiguousarray(stop_ids, dtype=np.uint32) if len(stop_ids) else np.zeros(1, np.uint32)
     out = np.zeros(max(max_new, 1), np.uint32)
     n = C.c_uint32()
@@ -623,15 +632,17 @@ def generate_sampled(model: Model, prompt_ids, max_new: int, sampler: Sampler, s
 
 
 def generate(model: Model, prompt_ids, max_new: int, stop_ids=(), max_ctx: int | None = None, keep_logits=False,
-             kv_dtype: int = 0):
+             kv_dtype: int = 0, window: int = 0, sinks: int = 0):
     """generate (src/generate.rs:83-157) with the greedy sampler
     (temperature 0): prefill once, then decode on the device.  Returns
-    (ids, per-step logits or None)."""
+    (ids, per-step logits or None).  window and sinks: KvCache.set_window."""
     p = np.ascontiguousarray(prompt_ids, dtype=np.uint32)
     max_ctx = max_ctx or min(model.config.context_length, 4096)
     if p.size + max_new > max_ctx:
         raise FurnaceError(FZ_EINVAL, f"prompt ({p.size}) + max tokens ({max_new}) exceeds context cap {max_ctx}")
     cache = KvCache(model, max_ctx, kv_dtype)
+    if window or sinks:
+        cache.set_window(window, sinks)
     logits, first = model.forward(p, cache, want_logits=keep_logits)
     ids, lg = model.decode_greedy(first, max_new, cache, stop_ids, keep_logits)
     if keep_logits:

@@ -199,6 +199,8 @@ struct KvQ8Attend {
   uint32_t window, sinks;
   float scale;
   void* work;  // kvq8_attend_work(c, b) bytes
+  void* runs = nullptr;  // one row only: its run records too, from record run0
+  uint32_t run0 = 0;
 };
 void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const void* k, const void* v, uint64_t ld,
                         cudaStream_t s);

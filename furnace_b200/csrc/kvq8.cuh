@@ -491,6 +491,8 @@ struct KqSplitArgs {
   uint64_t ldq, ldo;
   uint32_t window, sinks;
   float scale;          // softmax scale * log2(e)
+  XRun* runs;           // the result as run records too (every segment then goes through the merge), or null
+  uint32_t run0;
   uint64_t* prefix;     // [n_seqs + 1] cost before each sequence (written by CTA 0)
   float* slots;         // [2 * gridDim.x]
 };
@@ -723,7 +725,7 @@ __device__ __forceinline__ void kq_segment(const KqSplitArgs<HD, T>& a, KqSplitS
     for (int n = 0; n < HD / 8; n++)
       *reinterpret_cast<float2*>(&sm.acc[warp][g][n * 8 + 2 * t]) = make_float2(o[n][0], o[n][1]);
     __syncthreads();
-    const bool whole = nv == p.span.n;
+    const bool whole = nv == p.span.n && !a.runs;
     // a row is HD / 4 lanes, four dims each
     constexpr uint32_t L = HD / 4, RPP = KQ_SP_THREADS / L;  // lanes per row, rows per pass
 #pragma unroll
@@ -866,7 +868,7 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
   const uint64_t s0 = a.prefix[blockIdx.z] + (uint64_t)(kvh * p.groups + grp) * (p.span.n + KQ_SEG);
   const uint64_t s1 = s0 + p.span.n + KQ_SEG;
   const uint32_t i0 = (uint32_t)((s0 + KQ_SEG) / per), n = (uint32_t)((s1 - 1) / per) - i0 + 1;
-  if (n == 1) return;  // written by the run itself
+  if (n == 1 && !a.runs) return;  // written by the run itself
   __shared__ float wt[KQ_MG_PIECES];
   __shared__ float red[KQ_MG_THREADS / 32][HD], rden[KQ_MG_THREADS / 32], rtop[KQ_MG_THREADS / 32];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -903,11 +905,17 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 #pragma unroll
   for (int d = 0; d < DPL; d++) red[warp][lane * DPL + d] = acc[d];
   __syncthreads();
+  const uint32_t head = kvh * a.c.group + rr % a.c.group;
   if (tid < HD) {
     const float num = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
     den = (rden[0] + rden[1]) + (rden[2] + rden[3]);
-    kq_st(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + tid,
-          den == 0.f ? 0.f : __fdiv_rn(num, den));
+    const float y = den == 0.f ? 0.f : __fdiv_rn(num, den);
+    kq_st(a.out + (uint64_t)(p.s.row0 + j) * a.ldo + (uint64_t)head * HD + tid, y);
+    wt[tid] = y;
+  }
+  if (a.runs) {  // one row: the input of the o_proj GEMV
+    __syncthreads();
+    if (tid < HD) values_to_runs(wt, HD, nullptr, a.runs, a.run0 + head * (HD / 16), tid, HD);
   }
 }
 
@@ -1564,14 +1572,16 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
                        a.window,
                        a.sinks,
                        a.scale * 1.44269504088896341f,
+                       static_cast<XRun*>(a.runs),
+                       a.run0,
                        static_cast<uint64_t*>(a.work),
                        reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b))};
-  if (kvq8_by_rows(a.c, a.b)) {
+  if (!a.runs && kvq8_by_rows(a.c, a.b)) {
     const uint32_t tiles = (uint32_t)(((uint64_t)a.b.max_new * a.c.group + KR_M - 1) / KR_M);
     launch_pdl(k_kvq8_rows<HD, T>, dim3(tiles, a.c.nkv, a.b.n_seqs), dim3(KR_THREADS), sizeof(KrSmem<HD>), s, k);
     return;
   }
-  if (a.b.max_pages <= KQ_WHOLE_PAGES) {
+  if (!a.runs && a.b.max_pages <= KQ_WHOLE_PAGES) {
     const uint64_t groups = ((uint64_t)a.b.max_new * a.c.group + 7) / 8;
     launch_pdl(k_kvq8_whole<HD, T>, dim3((unsigned)(a.c.nkv * groups), a.b.n_seqs), dim3(KQ_SP_THREADS), smem, s, k);
     return;
@@ -1583,6 +1593,7 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
 
 void launch_kvq8_attend(const KvQ8Attend& a, cudaStream_t s) {
   if (!a.b.n_seqs) return;
+  if (a.runs && a.b.n_seqs * a.b.max_new != 1) fail(FZ_EINVAL, "run records are made for one row");
   if (a.c.hd == 128)
     a.f16 ? kvq8_attend_t<128, __half>(a, s) : kvq8_attend_t<128, float>(a, s);
   else

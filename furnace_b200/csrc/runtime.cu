@@ -119,7 +119,13 @@ struct fz_model {
 struct fz_kv {
   fz_model* m = nullptr;
   uint32_t max_ctx = 0, len = 0, splits = 0;
-  uint32_t eb = 4;  // bytes per cached element: 4 (f32) or 2 (f16)
+  uint32_t eb = 4;  // bytes per cached element: 4 (f32), 2 (f16) or 1 (8-bit codes)
+  // 8-bit codes (FZ_KV_Q8): k holds [layer][page][nkv_l][K|V][64][hd] bytes, v
+  // the scales [layer][page][nkv_l][K|V][4], a layer's page j its positions
+  // 64 j ..; attention over the last `window` positions (0: all) and the
+  // first `sinks`
+  uint32_t pages = 0, window = 0, sinks = 0;
+  bool q8() const { return eb == 1; }
   // layer li's K (or V) block [nkv_l][max_ctx][hd] of this rank
   void* layer_k(uint32_t li, uint32_t nkv, uint32_t hd) const {
     return k.as<uint8_t>() + (uint64_t)li * nkv * max_ctx * hd * eb;
@@ -127,13 +133,16 @@ struct fz_kv {
   void* layer_v(uint32_t li, uint32_t nkv, uint32_t hd) const {
     return v.as<uint8_t>() + (uint64_t)li * nkv * max_ctx * hd * eb;
   }
-  DevBuf k, v, rope_cs, partials, state, forced, ids;
-  cudaGraphExec_t g_full = nullptr, g_layers = nullptr;
-  // device memory and graphs back; the handle stays valid for fz_kv_free
-  void release() {
+  DevBuf k, v, rope_cs, partials, state, forced, ids;  // partials: the attention's work, whatever the element type
+  void drop_graphs() {
     if (g_full) cudaGraphExecDestroy(g_full);
     if (g_layers) cudaGraphExecDestroy(g_layers);
     g_full = g_layers = nullptr;
+  }
+  cudaGraphExec_t g_full = nullptr, g_layers = nullptr;
+  // device memory and graphs back; the handle stays valid for fz_kv_free
+  void release() {
+    drop_graphs();
     for (DevBuf* b : {&k, &v, &rope_cs, &partials, &state, &forced, &ids}) b->release();
   }
   ~fz_kv() { release(); }
@@ -456,6 +465,51 @@ AttnLaunch layer_attention(fz_kv* kv, uint32_t li, uint32_t splits) {
   return a;
 }
 
+// Layer li of an 8-bit cache as the paged kernels see it: one sequence whose
+// pages lie in order.
+KvQ8Dev q8_layer(const fz_kv* kv, uint32_t li, uint32_t* status) {
+  const fz_model* m = kv->m;
+  const uint64_t blocks = (uint64_t)kv->pages * m->nkv_l * 2;  // of 64 positions of one head's keys or values
+  return KvQ8Dev{kv->k.as<uint8_t>() + li * blocks * FZ_KVQ8_PAGE * m->cfg.head_dim,
+                 kv->v.as<float>() + li * blocks * (FZ_KVQ8_PAGE / FZ_KVQ8_BLOCK),
+                 kv->rope_cs.as<float2>(),
+                 status,
+                 kv->pages,
+                 kv->max_ctx,
+                 m->nkv_l,
+                 m->nh_l / m->nkv_l,
+                 m->cfg.head_dim};
+}
+
+// n positions of it that end at position `end` (0: at the step's own position).
+KvQ8Batch q8_rows(const fz_kv* kv, uint32_t n, uint32_t end) {
+  const StepState* st = kv->state.as<StepState>();
+  return KvQ8Batch{nullptr, end ? nullptr : reinterpret_cast<const int32_t*>(&st->pos), nullptr, 1, kv->pages, n, n,
+                   end ? (int32_t)end : 1};
+}
+
+// q, k and v rows [q | k | v], ldq apart, of the n positions that end at `end`:
+// k and v into layer li, then attention to ctx (and, for one row, its records).
+void q8_attention(fz_kv* kv, uint32_t li, uint32_t n, uint32_t end, const float* qkv, uint32_t ldq, float* ctx,
+                  uint32_t ldc, void* runs, uint32_t run0, uint32_t* status, cudaStream_t s) {
+  const fz_model* m = kv->m;
+  KvQ8Attend a{};
+  a.c = q8_layer(kv, li, status);
+  a.b = q8_rows(kv, n, end);
+  launch_kvq8_append(a.c, a.b, false, qkv + m->qd_l, qkv + m->qd_l + m->kd_l, ldq, s);
+  a.q = qkv;
+  a.out = ctx;
+  a.ldq = ldq;
+  a.ldo = ldc;
+  a.window = kv->window;
+  a.sinks = kv->sinks;
+  a.scale = 1.0f / sqrtf((float)m->cfg.head_dim);
+  a.work = kv->partials.p;
+  a.runs = runs;
+  a.run0 = run0;
+  launch_kvq8_attend(a, s);
+}
+
 // Sum of the ranks' residual-stream partials (tensor parallelism) where the
 // peer-memory exchange inside the GEMVs is unavailable (a rank could not
 // export its buffer, or FURNACE_B200_TP_ALLREDUCE=nccl): ncclAllReduce.
@@ -487,9 +541,12 @@ void record_step(fz_kv* kv, bool with_logits, cudaStream_t s, OpHook* hook = nul
     H(FZ_OP_QKV, true);
     launch_gemv(gl[4 * li], s);
     H(FZ_OP_QKV, false);
-    AttnLaunch a = layer_attention(kv, li, kv->splits);
     H(FZ_OP_ATTN, true);
-    launch_attention(a, s);
+    if (kv->q8())
+      q8_attention(kv, li, 1, 0, m->qkv.as<float>(), m->qd_l + 2 * m->kd_l, m->ctx.as<float>(), m->qd_l,
+                   m->runs_ctx[m->ctx_buf[li]]->p, m->o_off[li] / 16, st->pad, s);
+    else
+      launch_attention(layer_attention(kv, li, kv->splits), s);
     H(FZ_OP_ATTN, false);
     H(FZ_OP_OPROJ, true);
     launch_gemv(gl[4 * li + 1], s);
@@ -623,7 +680,10 @@ void prefill_tokens(fz_kv* kv, const uint32_t* tokens, uint32_t n, uint32_t pos0
       gemm(H, ldq, T, PE_STORE, m->pf_qkv.as<float>(), ldq, L.bqkv);
       // rotated k / v into the cache, causal attention per token
       if (L.wo.cols != qd) CK(cudaMemsetAsync(ctx, 0, (size_t)T * ldc * 4, s));
-      launch_prefill_attention(m->pf_qkv.as<float>(), ldq, kv->rope_cs.as<float>(), kv->layer_k(li, m->nkv_l, hd),
+      if (kv->q8())
+        q8_attention(kv, li, T, pos0 + c0 + T, m->pf_qkv.as<float>(), ldq, ctx + m->o_off[li], ldc, nullptr, 0, err, s);
+      else
+        launch_prefill_attention(m->pf_qkv.as<float>(), ldq, kv->rope_cs.as<float>(), kv->layer_k(li, m->nkv_l, hd),
                                kv->layer_v(li, m->nkv_l, hd), kv->eb == 2, ctx + m->o_off[li], ldc, m->nh_l,
                                m->nkv_l, hd, kv->max_ctx, pos0 + c0, T, err, s);
       // x += o_proj(ctx)
@@ -644,7 +704,8 @@ void prefill_tokens(fz_kv* kv, const uint32_t* tokens, uint32_t n, uint32_t pos0
   CK(cudaStreamSynchronize(s));
   if (e) {
     CK(cudaMemsetAsync(err, 0, 4, s));
-    fail(FZ_ETIMEOUT, "prefill: a bounded device wait ran out (code %u)", e);
+    // an 8-bit cache also notes values that are not finite; they end in the logits
+    if (e != KQ_NOT_FINITE) fail(FZ_ETIMEOUT, "prefill: a bounded device wait ran out (code %u)", e);
   }
 }
 
@@ -815,6 +876,10 @@ void check_state(fz_kv* kv) {
   // device wait (input records, ring slot, KV tile; residual exchange) ran out
   if (st.error >= 3) fail(FZ_ETIMEOUT, "a bounded device wait ran out (code %u)", st.error);
   if (st.error) fail(FZ_EINVAL, "device step rejected its input (code %u)", st.error);
+  // an 8-bit cache's status; values that are not finite end in the logits
+  const uint32_t q8 = st.pad[0] & ~(uint32_t)KQ_NOT_FINITE;
+  if (q8 & KQ_TIMEOUT) fail(FZ_ETIMEOUT, "a bounded device wait ran out");
+  if (q8) fail(FZ_EINVAL, "8-bit KV cache rejected its input (code %u)", q8);
 }
 
 void use_device(const fz_model* m) { CK(cudaSetDevice(m->device)); }
@@ -828,7 +893,10 @@ void step_bytes(const fz_model* m, const fz_kv* kv, uint64_t pos, double* bytes)
   for (auto& L : m->layers) {
     bytes[FZ_OP_QKV] += L.wq.gguf_bytes + L.wk.gguf_bytes + L.wv.gguf_bytes + (2 * H + qd + 2 * kd) * 4;
     bytes[FZ_OP_ROPE] += (qd + 2 * kd) * 4 + (qd + 2 * kd) * 4;
-    bytes[FZ_OP_ATTN] += 2 * (pos + 1) * kd * kv->eb + 2 * qd * 4;
+    uint64_t seen = pos + 1;  // positions the step attends to
+    if (kv->window && seen > kv->window) seen = kv->window + std::min<uint64_t>(kv->sinks, seen - kv->window);
+    bytes[FZ_OP_ATTN] += 2 * seen * kd * kv->eb + 2 * qd * 4;
+    if (kv->q8()) bytes[FZ_OP_ATTN] += 2 * seen * m->nkv_l * 4 / FZ_KVQ8_BLOCK;
     bytes[FZ_OP_OPROJ] += L.wo.gguf_bytes + (qd + 2 * H) * 4;
     bytes[FZ_OP_GATEUP] += L.wgu.gguf_bytes + (2 * H + F) * 4;
     bytes[FZ_OP_DOWN] += L.wd.gguf_bytes + (F + 2 * H) * 4;
@@ -1303,21 +1371,30 @@ int fz_model_stream(const fz_model* m, void** stream, int* device) {
 int fz_kv_new(fz_model* m, uint32_t max_ctx, int kv_dtype, fz_kv** out) {
   return guard([&] {
     need(m && out, "null argument");
-    need(kv_dtype == FZ_KV_F32 || kv_dtype == FZ_KV_F16, "kv dtype %d unsupported (FZ_KV_F32 or FZ_KV_F16)",
-         kv_dtype);
+    need(kv_dtype == FZ_KV_F32 || kv_dtype == FZ_KV_F16 || kv_dtype == FZ_KV_Q8,
+         "kv dtype %d unsupported (FZ_KV_F32, FZ_KV_F16 or FZ_KV_Q8)", kv_dtype);
     need(max_ctx > 0, "max_ctx must be positive");
     use_device(m);
     const fz_config& c = m->cfg;
     auto kv = std::make_unique<fz_kv>();
     kv->m = m;
     kv->max_ctx = max_ctx;
-    kv->eb = kv_dtype == FZ_KV_F16 ? 2 : 4;
-    uint64_t per = (uint64_t)c.n_layers * m->nkv_l * max_ctx * c.head_dim * kv->eb;  // this rank's KV heads
-    kv->k.alloc(per);
-    kv->v.alloc(per);
+    kv->eb = kv_dtype == FZ_KV_Q8 ? 1 : kv_dtype == FZ_KV_F16 ? 2 : 4;
     // every user of the cache runs on the model's stream
-    CK(cudaMemsetAsync(kv->k.p, 0, per, m->stream));
-    CK(cudaMemsetAsync(kv->v.p, 0, per, m->stream));
+    if (kv->q8()) {
+      need(max_ctx <= 0x7fffffffu - FZ_KVQ8_PAGE, "max_ctx %u unsupported", max_ctx);
+      kv->pages = (max_ctx + FZ_KVQ8_PAGE - 1) / FZ_KVQ8_PAGE;
+      const uint64_t blocks = (uint64_t)c.n_layers * kv->pages * m->nkv_l * 2;
+      kv->k.alloc(blocks * FZ_KVQ8_PAGE * c.head_dim);
+      kv->v.alloc(blocks * (FZ_KVQ8_PAGE / FZ_KVQ8_BLOCK) * 4);
+      CK(cudaMemsetAsync(kv->k.p, 128, kv->k.n, m->stream));  // code 0
+    } else {
+      uint64_t per = (uint64_t)c.n_layers * m->nkv_l * max_ctx * c.head_dim * kv->eb;  // this rank's KV heads
+      kv->k.alloc(per);
+      kv->v.alloc(per);
+      CK(cudaMemsetAsync(kv->k.p, 0, per, m->stream));
+    }
+    CK(cudaMemsetAsync(kv->v.p, 0, kv->v.n, m->stream));
     // RoPE factors with the reference's arithmetic (src/model.rs:207-210):
     // freq = theta^(-2i/hd), angle = pos * freq, (sin, cos) via libm.
     uint32_t half = c.head_dim / 2;
@@ -1334,7 +1411,8 @@ int fz_kv_new(fz_model* m, uint32_t max_ctx, int kv_dtype, fz_kv** out) {
     kv->rope_cs.alloc(cs.size() * 4);
     CK(cudaMemcpy(kv->rope_cs.p, cs.data(), cs.size() * 4, cudaMemcpyHostToDevice));
     kv->splits = attention_splits(m->nkv_l);
-    kv->partials.alloc(attention_partial_floats(m->nh_l, m->nkv_l, c.head_dim, kv->splits) * 4);
+    kv->partials.alloc(kv->q8() ? kvq8_attend_work(q8_layer(kv.get(), 0, nullptr), q8_rows(kv.get(), max_ctx, max_ctx))
+                                : attention_partial_floats(m->nh_l, m->nkv_l, c.head_dim, kv->splits) * 4);
     // the split-padding entries of the accumulator block are never written
     // and must read as zero (they are weighted by 0 in the merge)
     CK(cudaMemsetAsync(kv->partials.p, 0, kv->partials.n, m->stream));
@@ -1375,6 +1453,21 @@ int fz_kv_set_len(fz_kv* kv, uint32_t len) {
 
 int fz_kv_reset(fz_kv* kv) { return fz_kv_set_len(kv, 0); }
 
+int fz_kv_set_window(fz_kv* kv, uint32_t window, uint32_t sinks) {
+  return guard([&] {
+    need(kv != nullptr, "null kv");
+    need(kv->m != nullptr, "the cache's model has been freed");
+    need(kv->q8(), "a window needs an 8-bit cache (FZ_KV_Q8)");
+    need(window > 0 || sinks == 0, "%u sinks without a window", sinks);
+    if (window == kv->window && sinks == kv->sinks) return;
+    use_device(kv->m);
+    CK(cudaStreamSynchronize(kv->m->stream));  // the captured steps hold the old numbers
+    kv->drop_graphs();
+    kv->window = window;
+    kv->sinks = sinks;
+  });
+}
+
 int fz_kv_bytes(const fz_kv* kv, uint64_t* bytes) {
   return guard([&] {
     need(kv && bytes, "null argument");
@@ -1393,6 +1486,17 @@ int fz_kv_read(const fz_kv* kv, uint32_t layer, int which_v, uint32_t n, float* 
     CK(cudaStreamSynchronize(kv->m->stream));  // the copies below run on the legacy stream
     uint32_t hd = c.head_dim;
     const uint32_t nkv = kv->m->nkv_l;  // this rank's KV heads
+    if (kv->q8()) {
+      if (n == 0) return;
+      DevBuf rows((uint64_t)n * nkv * hd * 4), status(16);
+      cudaStream_t s = kv->m->stream;
+      CK(cudaMemsetAsync(status.p, 0, 16, s));
+      launch_kvq8_read(q8_layer(kv, layer, status.as<uint32_t>()), q8_rows(kv, n, n), false, which_v ? nullptr : rows.p,
+                       which_v ? rows.p : nullptr, nkv * hd, s);
+      CK(cudaMemcpyAsync(out, rows.p, (uint64_t)n * nkv * hd * 4, cudaMemcpyDeviceToHost, s));
+      CK(cudaStreamSynchronize(s));
+      return;
+    }
     const uint8_t* base = static_cast<const uint8_t*>(which_v ? kv->layer_v(layer, nkv, hd) : kv->layer_k(layer, nkv, hd));
     // device [kvh][pos][hd] -> host [pos][kvh*hd] (f16 elements widened exactly)
     const uint32_t eb = kv->eb;

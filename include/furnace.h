@@ -48,8 +48,10 @@ enum { FZ_F32 = 0, FZ_F16 = 1, FZ_Q5_0 = 6, FZ_Q8_0 = 8, FZ_Q4_K = 12, FZ_Q6_K =
 
 /* KV cache element types.  F32 is the reference's (src/model.rs:321-327);
  * F16 keeps binary16 elements, rounded to nearest even when appended (the
- * 8K-context cache of the 32B configuration: half the bytes per position). */
-enum { FZ_KV_F32 = 0, FZ_KV_F16 = 1 };
+ * 8K-context cache of the 32B configuration: half the bytes per position).
+ * Q8 keeps 8-bit codes with an f32 scale per 16 positions, KV head and side
+ * (fz_kvq8_append_dev below has the arithmetic): a quarter of f32's bytes. */
+enum { FZ_KV_F32 = 0, FZ_KV_F16 = 1, FZ_KV_Q8 = 2 };
 
 typedef struct fz_file fz_file;   /* GgufFile (src/gguf.rs:297-304) */
 typedef struct fz_model fz_model; /* Model (src/model.rs:511-517), resident in HBM */
@@ -145,7 +147,7 @@ int fz_tp_unique_id(void* id, size_t n);
 int fz_model_load_tp(const fz_file* f, int rank, int world, const void* id, size_t n, int device, fz_model** out);
 
 /* KvCache::new (src/model.rs:330-339): max_ctx positions of kv_dtype
- * (FZ_KV_F32 or FZ_KV_F16) elements. */
+ * (FZ_KV_F32, FZ_KV_F16 or FZ_KV_Q8) elements. */
 int fz_kv_new(fz_model* m, uint32_t max_ctx, int kv_dtype, fz_kv** out);
 /* Either order of fz_kv_free and fz_model_free is safe: freeing the model
  * releases its caches' device memory, and a cache handle of a freed model
@@ -157,7 +159,12 @@ int fz_kv_len(const fz_kv* kv, uint32_t* len);
 int fz_kv_set_len(fz_kv* kv, uint32_t len);
 /* kv.len = 0: the cache reused for a new sequence. */
 int fz_kv_reset(fz_kv* kv);
-/* KvCache::bytes (src/model.rs:341-343): K and V bytes of this rank's cache. */
+/* Attention over the last `window` positions and the first `sinks` only
+ * (window 0: over all, the default); no counterpart in the reference.  The
+ * cache keeps every position.  FZ_KV_Q8 caches only. */
+int fz_kv_set_window(fz_kv* kv, uint32_t window, uint32_t sinks);
+/* KvCache::bytes (src/model.rs:341-343): K and V bytes of this rank's cache
+ * (an 8-bit cache's scales among them). */
 int fz_kv_bytes(const fz_kv* kv, uint64_t* bytes);
 /* Copy layer `layer`'s cached K (which_v = 0) or V rows [0, n) to the host
  * as [n, n_kv_heads*head_dim] f32 (the reference's row layout); under tensor

@@ -817,7 +817,54 @@ struct KvCache {
   std::vector<std::vector<float>> k, v;
   size_t len = 0, max_ctx = 0, kv_dim = 0;
   bool f16 = false;  // elements kept as IEEE binary16 (rounded to nearest even when appended)
+  // 8-bit codes with a scale per 16 positions, head and side (no counterpart
+  // in the reference); k and v then hold code * scale.  Per layer: codes
+  // [2][max_ctx][kv_dim], scales [2][blocks][heads].
+  bool q8 = false;
+  size_t head_dim = 0, window = 0, sinks = 0;
+  std::vector<std::vector<int8_t>> codes;
+  std::vector<std::vector<float>> scales;
 };
+
+constexpr size_t Q8_BLOCK = 16;
+
+// Rows [start, start + n) of layer li's side (0 K, 1 V) quantized into the
+// cache: a block's scale is the largest magnitude of these rows in it / 127,
+// and at least the scale it has where it keeps older rows, which then take the
+// codes of the larger scale.
+void q8_append(KvCache* c, size_t li, int side, const float* x, size_t start, size_t n) {
+  const size_t kd = c->kv_dim, hd = c->head_dim, nh = kd / hd, nb = (c->max_ctx + Q8_BLOCK - 1) / Q8_BLOCK;
+  int8_t* codes = c->codes[li].data() + (size_t)side * c->max_ctx * kd;
+  float* scales = c->scales[li].data() + (size_t)side * nb * nh;
+  float* held = (side ? c->v : c->k)[li].data();
+  for (size_t b = start / Q8_BLOCK; b * Q8_BLOCK < start + n; b++) {
+    const size_t p0 = b * Q8_BLOCK, lo = std::max(start, p0), hi = std::min(start + n, p0 + Q8_BLOCK);
+    for (size_t h = 0; h < nh; h++) {
+      float top = 0.0f;
+      for (size_t p = lo; p < hi; p++)
+        for (size_t d = 0; d < hd; d++) top = std::max(top, fabsf(x[(p - start) * kd + h * hd + d]));
+      float& sc = scales[b * nh + h];
+      float s = top / 127.0f;
+      if (lo > p0) {
+        s = std::max(s, sc);
+        if (s > sc)
+          for (size_t p = p0; p < lo; p++)
+            for (size_t d = 0; d < hd; d++) {
+              int8_t& q = codes[p * kd + h * hd + d];
+              q = (int8_t)nearbyintf((float)q * (sc / s));
+            }
+      }
+      for (size_t p = lo; p < hi; p++)
+        for (size_t d = 0; d < hd; d++) {
+          const float v = x[(p - start) * kd + h * hd + d];
+          codes[p * kd + h * hd + d] = s > 0.0f ? (int8_t)std::min(127.0f, std::max(-127.0f, nearbyintf(v / s))) : 0;
+        }
+      sc = s;
+      for (size_t p = p0; p < hi; p++)
+        for (size_t d = 0; d < hd; d++) held[p * kd + h * hd + d] = (float)codes[p * kd + h * hd + d] * s;
+    }
+  }
+}
 
 // binary32 -> binary16, round to nearest even (overflow to infinity,
 // gradual underflow); the device's __float2half_rn rounding.
@@ -849,7 +896,7 @@ float round_to_half(float f) { return f16_to_f32(float_to_half_rne(f)); }
 // (src/model.rs:371-438); the uncached variants (:224-290) are the same
 // arithmetic with k/v taken from the current rows.
 void attention(const float* q, size_t n_new, const float* kc, const float* vc, size_t total, size_t start_pos,
-               size_t nh, size_t nkv, size_t hd, float* out) {
+               size_t nh, size_t nkv, size_t hd, float* out, size_t window = 0, size_t sinks = 0) {
   size_t kv_dim = nkv * hd, group = nh / nkv;
   float scale = 1.0f / sqrtf((float)hd);
   std::vector<float> probs(nh * n_new * total);
@@ -864,7 +911,7 @@ void attention(const float* q, size_t n_new, const float* kc, const float* vc, s
       const float* qh = q + s * nh * hd + h * hd;
       float* row = probs.data() + (h * n_new + s) * total;
       for (size_t t = 0; t < total; t++) {
-        if (t <= start_pos + s) {
+        if (t <= start_pos + s && (window == 0 || start_pos + s - t < window || t < sinks)) {
           const float* kh = kc + t * kv_dim + kv * hd;
           float d = 0.0f;
           for (size_t i = 0; i < hd; i++) d += qh[i] * kh[i];
@@ -907,10 +954,16 @@ void layer_forward(const float* x, size_t n_new, const Layer& L, const Config& c
         k[i] = round_to_half(k[i]);
         v[i] = round_to_half(v[i]);
       }
-    memcpy(cache->k[li].data() + start_pos * kd, k.data(), sizeof(float) * n_new * kd);
-    memcpy(cache->v[li].data() + start_pos * kd, v.data(), sizeof(float) * n_new * kd);
+    if (cache->q8) {
+      q8_append(cache, li, 0, k.data(), start_pos, n_new);
+      q8_append(cache, li, 1, v.data(), start_pos, n_new);
+    } else {
+      memcpy(cache->k[li].data() + start_pos * kd, k.data(), sizeof(float) * n_new * kd);
+      memcpy(cache->v[li].data() + start_pos * kd, v.data(), sizeof(float) * n_new * kd);
+    }
     size_t total = start_pos + n_new;
-    attention(q.data(), n_new, cache->k[li].data(), cache->v[li].data(), total, start_pos, nh, nkv, hd, ctx.data());
+    attention(q.data(), n_new, cache->k[li].data(), cache->v[li].data(), total, start_pos, nh, nkv, hd, ctx.data(),
+              cache->window, cache->sinks);
   } else {
     attention(q.data(), n_new, k.data(), v.data(), n_new, 0, nh, nkv, hd, ctx.data());
   }
@@ -1212,6 +1265,17 @@ void* orc_kv_new(void* mp, size_t max_ctx) {
 }
 void orc_kv_free(void* kv) { delete (KvCache*)kv; }
 void orc_kv_set_f16(void* kv, int on) { ((KvCache*)kv)->f16 = on != 0; }
+void orc_kv_set_q8(void* kvp, size_t head_dim) {
+  KvCache* kv = (KvCache*)kvp;
+  kv->q8 = true;
+  kv->head_dim = head_dim;
+  kv->codes.assign(kv->k.size(), std::vector<int8_t>(2 * kv->max_ctx * kv->kv_dim, 0));
+  kv->scales.assign(kv->k.size(), std::vector<float>(2 * ((kv->max_ctx + Q8_BLOCK - 1) / Q8_BLOCK) * (kv->kv_dim / head_dim), 0.0f));
+}
+void orc_kv_set_window(void* kv, size_t window, size_t sinks) {
+  ((KvCache*)kv)->window = window;
+  ((KvCache*)kv)->sinks = sinks;
+}
 uint16_t orc_float_to_half(float f) { return float_to_half_rne(f); }
 size_t orc_kv_len(void* kv) { return ((KvCache*)kv)->len; }
 void orc_kv_set_len(void* kv, size_t n) { ((KvCache*)kv)->len = n; }

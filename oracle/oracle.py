@@ -67,6 +67,8 @@ def lib():
             "orc_kv_new": (P, [P, S]),
             "orc_kv_free": (None, [P]),
             "orc_kv_set_f16": (None, [P, I]),
+            "orc_kv_set_q8": (None, [P, S]),
+            "orc_kv_set_window": (None, [P, S, S]),
             "orc_float_to_half": (C.c_uint16, [F]),
             "orc_kv_len": (S, [P]),
             "orc_kv_set_len": (None, [P, S]),
@@ -319,12 +321,19 @@ class KvCache:
 
     def __init__(self, model: Model, max_ctx: int, kv_dtype: int = 0):
         """kv_dtype 1: elements kept as IEEE binary16, rounded to nearest even
-        when appended (the device's FZ_KV_F16 cache); 0: f32 (the reference)."""
+        when appended (the device's FZ_KV_F16 cache); 2: 8-bit codes with a
+        scale per 16 positions, head and side (FZ_KV_Q8); 0: f32 (the reference)."""
         self.model = model
         self.max_ctx = max_ctx
         self._h = lib().orc_kv_new(model._h, max_ctx)
-        if kv_dtype:
+        if kv_dtype == 1:
             lib().orc_kv_set_f16(self._h, 1)
+        elif kv_dtype == 2:
+            lib().orc_kv_set_q8(self._h, model.head_dim)
+
+    def set_window(self, window: int, sinks: int = 0):
+        """Attention over the last `window` positions (0: all) and the first `sinks`."""
+        lib().orc_kv_set_window(self._h, window, sinks)
 
     def __del__(self):
         try:
