@@ -24,6 +24,7 @@
 
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>

@@ -206,6 +206,7 @@ void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const vo
                         cudaStream_t s);
 void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, void* v, uint64_t ld, cudaStream_t s);
 uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b);
+uint64_t kvq8_attend_work_most(const KvQ8Dev& c, uint32_t n_seqs);  // whatever the sequences' rows and pages
 void launch_kvq8_attend(const KvQ8Attend& a, cudaStream_t s);
 
 }  // namespace fz

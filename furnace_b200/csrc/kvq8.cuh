@@ -494,7 +494,8 @@ struct KqSplitArgs {
   XRun* runs;           // the result as run records too (every segment then goes through the merge), or null
   uint32_t run0;
   uint64_t* prefix;     // [n_seqs + 1] cost before each sequence (written by CTA 0)
-  float* slots;         // [2 * gridDim.x]
+  float* slots;         // [2 * gridDim.x]; k_kvq8_rows: the parts' results, kr_part_floats each
+  uint32_t parts;       // k_kvq8_rows: CTAs of the same rows
 };
 
 // Rows of one segment: 16 threads a row, each N pairs.  get() starts the
@@ -951,6 +952,10 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 // low parts.  P's positions go in the order of the value bytes (2t, 2t + 1, 8 +
 // 2t, 9 + 2t for t = 0..3 of a block), which makes its pairs neighbours and the
 // conversion of the values a plain copy.
+//
+// Where a call has fewer CTAs than the GPU has SMs, the steps of a CTA's rows
+// are cut into `parts` of about equal length, a CTA each, whose results
+// k_kvq8_join joins.
 // ---------------------------------------------------------------------------
 constexpr uint32_t KR_M = 128;
 constexpr uint32_t KR_THREADS = 512;
@@ -968,7 +973,7 @@ struct KrSmem {
   __half qh[KR_M * HD], ql[KR_M * HD], k[2][KR_POS * HD], v[2][KR_POS * HD];
   float rowf[KR_M], l[2][KR_M], last[2][KR_M], m[2][KR_M], alpha[4][KR_M];
   uint32_t rowpos[KR_M];
-  uint64_t k_full[2], v_full[2], s_full[KR_NS], m_full[2], a_full[4], p_full[KR_NS], o_full, o_free, l_full, fin;
+  uint64_t k_full[2], v_full[2], s_full[KR_NS], m_full[2], a_full[4], p_full[KR_NS], o_full, o_free, l_full, q_full, fin;
   uint32_t tmem;
 };
 
@@ -1043,6 +1048,12 @@ __device__ __forceinline__ uint32_t kr_bits(uint32_t base, uint32_t lo, uint32_t
   const uint32_t a = lo > base ? min(lo - base, 32u) : 0u, b = hi > base ? min(hi - base, 32u) : 0u;
   const uint32_t below_b = b >= 32 ? 0xffffffffu : (1u << b) - 1, below_a = a >= 32 ? 0xffffffffu : (1u << a) - 1;
   return below_b & ~below_a;
+}
+
+// A part's result: the rows' sums, maxima and denominators.
+template <int HD>
+__host__ __device__ constexpr uint32_t kr_part_floats() {
+  return KR_M * HD + 2 * KR_M;
 }
 
 // Page numbers of 32 pages, one per lane, and of the 32 after them.
@@ -1122,13 +1133,26 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   pdl_wait();
   const KqSeq s = kq_plan(a.c, a.b, seq, 0, 0).s;
   const uint32_t nrows = (uint32_t)s.n_new * a.c.group, tiles = (nrows + KR_M - 1) / KR_M;
-  if (blockIdx.x >= tiles) return;
-  const uint32_t r0 = (tiles - 1 - blockIdx.x) * KR_M;  // the longest first
+  const uint32_t part = blockIdx.x % a.parts, tile = tiles - 1 - blockIdx.x / a.parts;  // the longest first
+  if (blockIdx.x / a.parts >= tiles) return;
+  const uint32_t r0 = tile * KR_M;
   const uint32_t p0 = s.len - s.n_new;
   const uint32_t plo = p0 + r0 / a.c.group, phi = p0 + min(r0 + KR_M - 1, nrows - 1) / a.c.group;
   const KqSpan span = kq_span(plo, phi, a.window, a.sinks);
+  const uint32_t all = (span.n + 1) / 2, step0 = (uint32_t)((uint64_t)all * part / a.parts);
+  const uint32_t steps = (uint32_t)((uint64_t)all * (part + 1) / a.parts) - step0;  // of this CTA
+  float* slot = a.slots + (((uint64_t)(seq * a.c.nkv + kvh) * (gridDim.x / a.parts) + tile) * a.parts + part) *
+                              kr_part_floats<HD>();
+  if (steps == 0) {  // only where there are parts
+    if (tid < KR_M) {
+      slot[KR_M * HD + tid] = -INFINITY;
+      slot[KR_M * HD + KR_M + tid] = 0.f;
+    }
+    return;
+  }
+  // page i of this CTA's steps; one past the last is the last again
   auto page_of = [&](uint32_t i) {
-    return (uint32_t)max(kq_page(a.c, a.b, seq, span.page(min(i, span.n - 1))), 0);
+    return (uint32_t)max(kq_page(a.c, a.b, seq, span.page(min(2 * step0 + i, span.n - 1))), 0);
   };
 
   if (tid == 0) {
@@ -1145,6 +1169,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     mbar_init(&sm.o_full, 1);
     mbar_init(&sm.o_free, KR_M);
     mbar_init(&sm.l_full, 2 * KR_M);
+    mbar_init(&sm.q_full, 256);
     mbar_init(&sm.fin, 1);
     fence_barrier_init();
   }
@@ -1152,54 +1177,6 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  // the rows, rotated, scaled to 2^13 and split, 16 threads a row
-  {
-    constexpr uint32_t N = half / 16;
-    for (uint32_t r = tid >> 4; r < KR_M; r += KR_THREADS / 16) {  // whole warps
-      const uint32_t rr = r0 + r, j = rr / a.c.group, l16 = tid & 15, d = l16 * N;
-      float x[2 * N] = {}, top = 0.f;
-      if (rr < nrows) {
-        const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + d;
-        kq_ldn<N>(p, x);
-        kq_ldn<N>(p + half, x + N);
-        if (a.c.rope) {
-          float f[2 * N];
-          const float* cs = reinterpret_cast<const float*>(a.c.rope + (uint64_t)(p0 + j) * half + d);
-          kq_ldn<N>(cs, f);
-          kq_ldn<N>(cs + N, f + N);
-#pragma unroll
-          for (uint32_t i = 0; i < N; i++) {
-            const float u = x[i], w = x[N + i];
-            x[i] = __fsub_rn(__fmul_rn(u, f[2 * i]), __fmul_rn(w, f[2 * i + 1]));
-            x[N + i] = __fadd_rn(__fmul_rn(u, f[2 * i + 1]), __fmul_rn(w, f[2 * i]));
-          }
-        }
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 2 * N; i++) top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int e = max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
-      // a negative softmax scale turns the row, so that factors are not negative
-      const float up = copysignf(__uint_as_float((uint32_t)(127 + 13 - e) << 23), a.scale);
-#pragma unroll
-      for (uint32_t k = 0; k < 2; k++)
-#pragma unroll
-        for (uint32_t i = 0; i < N; i += 2) {
-          const uint32_t at = panel_elem(KR_M, r, k * half + d + i);
-          const float u = x[k * N + i] * up, w = x[k * N + i + 1] * up;
-          const __half2 h = __floats2half2_rn(u, w);
-          const float2 g = __half22float2(h);
-          *reinterpret_cast<__half2*>(&sm.qh[at]) = h;
-          *reinterpret_cast<uint32_t*>(&sm.ql[at]) = kq_pack(u - g.x, w - g.y);
-        }
-      if (l16 == 0) {
-        sm.rowf[r] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-        sm.rowpos[r] = rr < nrows ? p0 + j : phi;  // a row that is none: zeros, not written
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -1215,7 +1192,6 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     constexpr uint32_t n = sizeof(bar) / sizeof(uint64_t);
     return mbar_wait(reinterpret_cast<uint64_t*>(&bar) + i % n, (i / n) & 1);
   };
-  const uint32_t steps = (span.n + 1) / 2;
 
   if (warp >= 12) kr_regs_dec<KR_REG_OTHER>();
   if (warp == 15) {
@@ -1231,6 +1207,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
                       kr_idesc<KR_POS>(), part || ks);
         umma_commit(&sm.s_full[i % KR_NS]);
       };
+      ok = mbar_wait(&sm.q_full, 0);
       for (uint32_t i = 0; i < min(2u, steps) && ok; i++) {
         ok = wait(sm.k_full, i);
         if (ok) scores(i);
@@ -1370,23 +1347,110 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       mbar_arrive(&sm.o_free);
     }
     ok = ok && mbar_wait(&sm.l_full, 0);
-    const uint32_t rr = r0 + row;
-    if (ok && rr < nrows) {
-      // each warpgroup's denominator goes by the maximum of its own last step; the sums by that of the last
+    // The result goes out through shared memory (the operands': every product is done), a warp a row at a time.  Each
+    // warpgroup's denominator goes by the maximum of its own last step, the sums by that of the last.
+    if (ok) {
       const float m0 = sm.last[0][row], m1 = sm.last[1][row], top = fmaxf(m0, m1);
       const float l = (m0 == -INFINITY ? 0.f : sm.l[0][row] * kq_exp2(m0 - top)) +
                       (m1 == -INFINITY ? 0.f : sm.l[1][row] * kq_exp2(m1 - top));
-      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
-      T* out = a.out + (uint64_t)(s.row0 + rr / a.c.group) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD;
+      float inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
+      if (a.parts > 1) {
+        inv = 1.f / KR_P;
+        slot[KR_M * HD + row] = top;
+        slot[KR_M * HD + KR_M + row] = l;
+      }
+      constexpr uint32_t ST = HD + 4;  // floats of a row: rows start in different banks
+      static_assert(KR_M * ST * 4 <= sizeof(sm.k) + sizeof(sm.v), "room for the result");
+      float* tile = reinterpret_cast<float*>(&sm.k[0][0]) + (warp & 3) * 32 * ST;  // this warp's 32 rows
 #pragma unroll
       for (int d = 0; d < HD; d += 4) {
 #pragma unroll
         for (int k = 0; k < 4; k++) acc[d + k] = l == 0.f ? 0.f : acc[d + k] * inv;
-        kq_st4(out + d, acc + d);
+        kq_st4(tile + lane * ST + d, acc + d);
+      }
+      __syncwarp();
+      constexpr uint32_t L = HD / 4, RP = 32 / L;  // lanes of a row, rows at a time
+      const uint32_t mine = r0 + row, j = mine / a.c.group;
+      const uint64_t off = (uint64_t)(s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + mine - j * a.c.group) * HD;
+      const uint32_t first = (warp & 3) * 32, live = nrows > r0 + first ? min(nrows - r0 - first, 32u) : 0;
+#pragma unroll 4
+      for (uint32_t r = 0; r < 32; r += RP) {
+        const uint32_t at = r + lane / L, d = lane % L * 4;
+        const uint64_t to = __shfl_sync(0xffffffffu, off, at);
+        float v[4];
+        kq_ldn<4>(tile + at * ST + d, v);
+        if (at >= live) continue;
+        if (a.parts > 1)
+          kq_st4(slot + (first + at) * HD + d, v);
+        else
+          kq_st4(a.out + to + d, v);
       }
     }
   } else {
     kr_regs_dec<KR_REG_OTHER>();
+    // The rows, rotated, scaled to 2^13 and split.  A warp takes eight rows, a lane 8 dims of one at a time (and the 8
+    // they are paired with): eight lanes then store one core matrix.
+    {
+      constexpr uint32_t CH = half / 32;
+#pragma unroll 1
+      for (uint32_t rg = warp; rg < KR_M / 8; rg += 8) {
+        const uint32_t r = rg * 8 + (lane & 7), rr = r0 + r, j = rr / a.c.group;
+        const T* p = a.q + (uint64_t)(s.row0 + j) * a.ldq + (uint64_t)(kvh * a.c.group + rr - j * a.c.group) * HD;
+        const float* cs = reinterpret_cast<const float*>(a.c.rope + (uint64_t)(p0 + j) * half);
+        float x[CH][16], f[CH][16], top = 0.f;
+#pragma unroll
+        for (uint32_t ch = 0; ch < CH; ch++) {
+          const uint32_t d = (lane >> 3) * 8 + ch * 32;
+#pragma unroll
+          for (uint32_t i = 0; i < 16; i++) x[ch][i] = 0.f, f[ch][i] = i % 2 ? 0.f : 1.f;
+          if (rr < nrows) {
+            kq_ldn<8>(p + d, x[ch]);
+            kq_ldn<8>(p + half + d, x[ch] + 8);
+            if (a.c.rope) kq_ldn<16>(cs + 2 * d, f[ch]);
+          }
+        }
+#pragma unroll
+        for (uint32_t ch = 0; ch < CH; ch++)
+#pragma unroll
+          for (uint32_t i = 0; i < 8; i++) {
+            const float u = x[ch][i], w = x[ch][8 + i];
+            if (a.c.rope) {
+              x[ch][i] = __fsub_rn(__fmul_rn(u, f[ch][2 * i]), __fmul_rn(w, f[ch][2 * i + 1]));
+              x[ch][8 + i] = __fadd_rn(__fmul_rn(u, f[ch][2 * i + 1]), __fmul_rn(w, f[ch][2 * i]));
+            }
+            top = fmaxf(top, fmaxf(fabsf(x[ch][i]), fabsf(x[ch][8 + i])));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const int e = max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
+        // a negative softmax scale turns the row, so that factors are not negative
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 13 - e) << 23), a.scale);
+#pragma unroll
+        for (uint32_t ch = 0; ch < CH; ch++)
+#pragma unroll
+          for (uint32_t k = 0; k < 2; k++) {
+            const uint32_t kc = (lane >> 3) + ch * 4 + k * (half / 8), at = (kc * (KR_M / 8) + rg) * 64 + (lane & 7) * 8;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              const float u = x[ch][8 * k + 2 * i] * up, w = x[ch][8 * k + 2 * i + 1] * up;
+              const __half2 h = __floats2half2_rn(u, w);
+              const float2 g = __half22float2(h);
+              hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+              lo[i] = kq_pack(u - g.x, w - g.y);
+            }
+            *reinterpret_cast<uint4*>(&sm.qh[at]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(&sm.ql[at]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        if (lane < 8) {
+          sm.rowf[r] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+          sm.rowpos[r] = rr < nrows ? p0 + j : phi;  // a row that is none: zeros, not written
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&sm.q_full);
+    }
+    ok = __all_sync(0xffffffffu, mbar_wait(&sm.q_full, 0));
     const uint32_t row = tid & 127, wg = warp >> 2, lanes = ((warp & 3) * 32) << 16, side = lane >> 2 & 1;
     const float rowf = sm.rowf[row];
     const uint32_t rowpos = sm.rowpos[row];
@@ -1400,7 +1464,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     float ks_next, vs_next;
     scales(page_of(2 * wg + side), &ks_next, &vs_next);
     uint32_t next = page_of(2 * wg + 4 + side);
-    for (uint32_t i = wg; i < steps; i += 2) {
+    for (uint32_t i = wg; i < steps && ok; i += 2) {
       const float ks = ks_next, vs = vs_next, lv = __log2f(fmaxf(vs, KQ_MIN_SCALE));
       scales(next, &ks_next, &vs_next);
       next = page_of(2 * i + 8 + side);
@@ -1408,8 +1472,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       if (!ok) break;
       tc_fence_after();
       const uint32_t t = tm + lanes + KR_S + i % KR_NS * KR_POS;
-      const bool none = 2 * i + 1 >= span.n;  // the last step has one page
-      const uint32_t pos[2] = {span.page(2 * i) * KQ_PAGE, span.page(2 * i + 1) * KQ_PAGE};
+      const uint32_t at = 2 * (step0 + i);
+      const bool none = at + 1 >= span.n;  // the last step has one page
+      const uint32_t pos[2] = {span.page(at) * KQ_PAGE, span.page(at + 1) * KQ_PAGE};
       bool masked = none;
 #pragma unroll
       for (int k = 0; k < 2; k++)
@@ -1485,6 +1550,42 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
 }
 
+// Join the parts of k_kvq8_rows: a warp a row, a lane HD / 32 dims.  Grid (rows
+// of a KV head / 4, nkv, n_seqs).
+constexpr int KR_JOIN_THREADS = 128;
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(KR_JOIN_THREADS) k_kvq8_join(const __grid_constant__ KqSplitArgs<HD, T> a,
+                                                               uint32_t tiles) {
+  pdl_trigger();
+  pdl_wait();
+  const KqSeq s = kq_plan(a.c, a.b, blockIdx.z, 0, 0).s;
+  const uint32_t rr = blockIdx.x * (KR_JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t kvh = blockIdx.y, j = rr / a.c.group, row = rr % KR_M;
+  if (j >= (uint32_t)s.n_new) return;
+  const float* slot = a.slots + ((uint64_t)(blockIdx.z * a.c.nkv + kvh) * tiles + rr / KR_M) * a.parts *
+                                    kr_part_floats<HD>();
+  float top = -INFINITY;
+  for (uint32_t i = 0; i < a.parts; i++) top = fmaxf(top, slot[(uint64_t)i * kr_part_floats<HD>() + KR_M * HD + row]);
+  constexpr int DPL = HD / 32;
+  float acc[DPL] = {}, den = 0.f;
+#pragma unroll 4
+  for (uint32_t i = 0; i < a.parts; i++) {
+    const float* p = slot + (uint64_t)i * kr_part_floats<HD>();
+    const float m = p[KR_M * HD + row];
+    if (m == -INFINITY) continue;  // nothing seen: its sums may not be there
+    const float f = kq_exp2(m - top);
+    float x[DPL];
+    kq_ldn<DPL>(p + row * HD + lane * DPL, x);
+    den = fmaf(f, p[KR_M * HD + KR_M + row], den);
+#pragma unroll
+    for (int d = 0; d < DPL; d++) acc[d] = fmaf(f, x[d], acc[d]);
+  }
+  T* out = a.out + (uint64_t)(s.row0 + j) * a.ldo + (uint64_t)(kvh * a.c.group + rr % a.c.group) * HD + lane * DPL;
+#pragma unroll
+  for (int d = 0; d < DPL; d++) kq_st(out + d, den == 0.f ? 0.f : __fdiv_rn(acc[d], den));
+}
+
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
@@ -1541,16 +1642,44 @@ static uint32_t kvq8_runs(const KvQ8Dev& c, const KvQ8Batch& b) {
 }
 static uint64_t kvq8_prefix_bytes(const KvQ8Batch& b) { return ((uint64_t)b.n_seqs + 1) * 8 + 15 & ~15ull; }
 
-// Many rows go to k_kvq8_rows.  It reads a page once for 128 rows, but a
-// sequence's rows walk all their pages one after the other, so there have to
-// be row groups enough for the split form to take longer.
-static bool kvq8_by_rows(const KvQ8Dev& c, const KvQ8Batch& b) {
-  const uint64_t rows = (uint64_t)b.max_new * c.group;
-  return rows >= 64 && b.n_seqs * c.nkv * ((rows + 7) / 8) >= 256;
+// CTAs of the same rows: enough to fill the SMs, each with two steps (four
+// pages) or more of the longest sequence there can be.
+static uint32_t kvq8_tiles(const KvQ8Dev& c, const KvQ8Batch& b) {
+  return (uint32_t)(((uint64_t)b.max_new * c.group + KR_M - 1) / KR_M);
+}
+static uint32_t kvq8_parts(const KvQ8Dev& c, const KvQ8Batch& b) {
+  const uint64_t ctas = (uint64_t)kvq8_tiles(c, b) * c.nkv * b.n_seqs;
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)num_sms() / ctas, b.max_pages / 4));
 }
 
+// Whether the call's rows go to k_kvq8_rows or to the split form, by the time
+// that each takes for the longest sequence there can be: a step of two pages of
+// 128 rows (fewer cost the same) takes k_kvq8_rows 2 us an SM, a page of 8 rows
+// the split form 2.8 ns with all SMs at work; starting and joining takes 17 and
+// 7.  Measured (us, split / rows): 1 sequence, 20 rows x 7 heads on 1000
+// positions 13.8 / 21.4, 100 rows on 2000 46 / 28, 512 rows on 3000 288 / 71;
+// 12 x 6 rows on up to 3000 37 / 63.
+static bool kvq8_by_rows(const KvQ8Dev& c, const KvQ8Batch& b) {
+  const double pages = b.max_pages, groups = (double)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8);
+  const double waves = std::ceil((double)kvq8_tiles(c, b) * c.nkv * b.n_seqs / num_sms());
+  return 17.0 + pages * waves / kvq8_parts(c, b) < 7.0 + 0.0028 * groups * pages;
+}
+
+static uint64_t kvq8_part_bytes(const KvQ8Dev& c) { return (uint64_t)(KR_M * c.hd + 2 * KR_M) * 4; }
+static uint64_t kvq8_split_bytes(const KvQ8Dev& c, uint64_t runs) { return 2 * runs * (8 * c.hd + 16) * 4; }
+
 uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b) {
-  return kvq8_prefix_bytes(b) + 2ull * kvq8_runs(c, b) * (8 * c.hd + 16) * 4;
+  if (!b.n_seqs) return 16;
+  if (!kvq8_by_rows(c, b)) return kvq8_prefix_bytes(b) + kvq8_split_bytes(c, kvq8_runs(c, b));
+  const uint64_t parts = kvq8_parts(c, b);
+  return parts == 1 ? 16 : (uint64_t)kvq8_tiles(c, b) * c.nkv * b.n_seqs * parts * kvq8_part_bytes(c);
+}
+
+uint64_t kvq8_attend_work_most(const KvQ8Dev& c, uint32_t n_seqs) {
+  KvQ8Batch b{};
+  b.n_seqs = n_seqs;
+  // parts are made only where they and the rows' tiles fit the SMs
+  return std::max(kvq8_prefix_bytes(b) + kvq8_split_bytes(c, KQ_MG_PIECES), num_sms() * kvq8_part_bytes(c));
 }
 
 template <int HD, typename T>
@@ -1575,10 +1704,17 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
                        static_cast<XRun*>(a.runs),
                        a.run0,
                        static_cast<uint64_t*>(a.work),
-                       reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b))};
+                       reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b)),
+                       1};
   if (!a.runs && kvq8_by_rows(a.c, a.b)) {
-    const uint32_t tiles = (uint32_t)(((uint64_t)a.b.max_new * a.c.group + KR_M - 1) / KR_M);
-    launch_pdl(k_kvq8_rows<HD, T>, dim3(tiles, a.c.nkv, a.b.n_seqs), dim3(KR_THREADS), sizeof(KrSmem<HD>), s, k);
+    const uint32_t tiles = kvq8_tiles(a.c, a.b);
+    k.parts = kvq8_parts(a.c, a.b);
+    k.slots = static_cast<float*>(a.work);
+    launch_pdl(k_kvq8_rows<HD, T>, dim3(tiles * k.parts, a.c.nkv, a.b.n_seqs), dim3(KR_THREADS), sizeof(KrSmem<HD>), s,
+               k);
+    if (k.parts > 1)
+      launch_pdl(k_kvq8_join<HD, T>, dim3((a.b.max_new * a.c.group + 3) / 4, a.c.nkv, a.b.n_seqs),
+                 dim3(KR_JOIN_THREADS), 0, s, k, tiles);
     return;
   }
   if (!a.runs && a.b.max_pages <= KQ_WHOLE_PAGES) {

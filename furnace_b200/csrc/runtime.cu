@@ -1411,7 +1411,7 @@ int fz_kv_new(fz_model* m, uint32_t max_ctx, int kv_dtype, fz_kv** out) {
     kv->rope_cs.alloc(cs.size() * 4);
     CK(cudaMemcpy(kv->rope_cs.p, cs.data(), cs.size() * 4, cudaMemcpyHostToDevice));
     kv->splits = attention_splits(m->nkv_l);
-    kv->partials.alloc(kv->q8() ? kvq8_attend_work(q8_layer(kv.get(), 0, nullptr), q8_rows(kv.get(), max_ctx, max_ctx))
+    kv->partials.alloc(kv->q8() ? kvq8_attend_work_most(q8_layer(kv.get(), 0, nullptr), 1)
                                 : attention_partial_floats(m->nh_l, m->nkv_l, c.head_dim, kv->splits) * 4);
     // the split-padding entries of the accumulator block are never written
     // and must read as zero (they are weighted by 0 in the merge)
