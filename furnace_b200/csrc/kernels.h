@@ -201,9 +201,12 @@ struct KvQ8Attend {
   void* work;  // kvq8_attend_work(c, b) bytes
   void* runs = nullptr;  // one row only: its run records too, from record run0
   uint32_t run0 = 0;
+  // the launch before it on the stream is launch_kvq8_append of the same rows,
+  // one a sequence, with late = true: reading older pages need not wait for it
+  bool after_append = false;
 };
 void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const void* k, const void* v, uint64_t ld,
-                        cudaStream_t s);
+                        cudaStream_t s, bool late = false);
 void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, void* v, uint64_t ld, cudaStream_t s);
 uint64_t kvq8_attend_work(const KvQ8Dev& c, const KvQ8Batch& b);
 uint64_t kvq8_attend_work_most(const KvQ8Dev& c, uint32_t n_seqs);  // whatever the sequences' rows and pages

@@ -151,9 +151,10 @@ __device__ __forceinline__ void kq_ldn(const __half* p, float* x) {
 // ---------------------------------------------------------------------------
 template <int HD, typename T>
 __global__ void __launch_bounds__(HD) k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k,
-                                                    const T* __restrict__ v, uint64_t ld) {
-  pdl_trigger();
+                                                    const T* __restrict__ v, uint64_t ld, bool late) {
+  if (!late) pdl_trigger();
   pdl_wait();
+  if (late) pdl_trigger();  // what comes next may read what this kernel's predecessors wrote before it waits
   const KqSeq s = kq_seq(b, blockIdx.z, c.status);
   const int32_t p0 = s.len - s.n_new;
   const int32_t blk = p0 / (int32_t)KQ_BLOCK + (int32_t)blockIdx.x, base = blk * (int32_t)KQ_BLOCK;
@@ -496,6 +497,7 @@ struct KqSplitArgs {
   uint64_t* prefix;     // [n_seqs + 1] cost before each sequence (written by CTA 0)
   float* slots;         // [2 * gridDim.x]; k_kvq8_rows: the parts' results, kr_part_floats each
   uint32_t parts;       // k_kvq8_rows: CTAs of the same rows
+  uint32_t after;       // k_kvq8_split: the predecessor is an append (late) of the batch's rows
 };
 
 // Rows of one segment: 16 threads a row, each N pairs.  get() starts the
@@ -766,7 +768,9 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
   extern __shared__ __align__(128) uint8_t smem_raw[];
   KqSplitSmem<HD>& sm = *reinterpret_cast<KqSplitSmem<HD>*>(smem_raw);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_wait();
+  // Behind an append of the same rows only the CTAs that read the pages it wrote wait for it: those that go up to a
+  // sequence's end (one new row, so the last page alone).
+  if (!a.after) pdl_wait();
   pdl_trigger();  // after the wait: what the merge reads of the inputs is final when it starts
   // this CTA's run [w0, w1) of the call's cost and the sequence it starts in
   uint64_t total = 0, mine = 0;  // mine: the cost of sequence tid
@@ -831,6 +835,7 @@ __global__ void __launch_bounds__(KQ_SP_THREADS, KQ_SP_CTAS) k_kvq8_split(const 
     const uint32_t u1 = (uint32_t)min((uint64_t)len, u0 + (w1 - w));
     const uint32_t v0 = max(u0, KQ_SEG) - KQ_SEG, v1 = max(u1, KQ_SEG) - KQ_SEG;
     if (v1 > v0) {
+      if (a.after && v1 == p.span.n) pdl_wait();
       // a run has at most two pieces that are not whole segments: its first and its last
       kq_segment<HD, T>(a, sm, p, seq, seg / p.groups, seg % p.groups, v0, v1 - v0,
                         a.slots + (2ull * blockIdx.x + (w != w0)) * kq_slot_floats<HD>());
@@ -1593,20 +1598,20 @@ __global__ void __launch_bounds__(KR_JOIN_THREADS) k_kvq8_join(const __grid_cons
 static uint32_t kvq8_blocks(const KvQ8Batch& b) { return (b.max_new + 2 * KQ_BLOCK - 2) / KQ_BLOCK; }
 
 template <int HD, typename T>
-static void kvq8_append_t(const KvQ8Dev& c, const KvQ8Batch& b, const void* k, const void* v, uint64_t ld,
+static void kvq8_append_t(const KvQ8Dev& c, const KvQ8Batch& b, const void* k, const void* v, uint64_t ld, bool late,
                           cudaStream_t s) {
   const dim3 grid(kvq8_blocks(b), c.nkv, b.n_seqs);
   launch_pdl(k_kvq8_append<HD, T>, grid, dim3(HD), 0, s, c, b, static_cast<const T*>(k),
-             static_cast<const T*>(v), ld);
+             static_cast<const T*>(v), ld, late);
 }
 
 void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const void* k, const void* v, uint64_t ld,
-                        cudaStream_t s) {
+                        cudaStream_t s, bool late) {
   if (!b.n_seqs) return;
   if (c.hd == 128)
-    f16 ? kvq8_append_t<128, __half>(c, b, k, v, ld, s) : kvq8_append_t<128, float>(c, b, k, v, ld, s);
+    f16 ? kvq8_append_t<128, __half>(c, b, k, v, ld, late, s) : kvq8_append_t<128, float>(c, b, k, v, ld, late, s);
   else
-    f16 ? kvq8_append_t<64, __half>(c, b, k, v, ld, s) : kvq8_append_t<64, float>(c, b, k, v, ld, s);
+    f16 ? kvq8_append_t<64, __half>(c, b, k, v, ld, late, s) : kvq8_append_t<64, float>(c, b, k, v, ld, late, s);
 }
 
 template <int HD, typename T>
@@ -1705,7 +1710,8 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
                        a.run0,
                        static_cast<uint64_t*>(a.work),
                        reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + kvq8_prefix_bytes(a.b)),
-                       1};
+                       1,
+                       a.after_append};
   if (!a.runs && kvq8_by_rows(a.c, a.b)) {
     const uint32_t tiles = kvq8_tiles(a.c, a.b);
     k.parts = kvq8_parts(a.c, a.b);

@@ -496,7 +496,8 @@ void q8_attention(fz_kv* kv, uint32_t li, uint32_t n, uint32_t end, const float*
   KvQ8Attend a{};
   a.c = q8_layer(kv, li, status);
   a.b = q8_rows(kv, n, end);
-  launch_kvq8_append(a.c, a.b, false, qkv + m->qd_l, qkv + m->qd_l + m->kd_l, ldq, s);
+  a.after_append = runs != nullptr;  // a decode step: one row
+  launch_kvq8_append(a.c, a.b, false, qkv + m->qd_l, qkv + m->qd_l + m->kd_l, ldq, s, a.after_append);
   a.q = qkv;
   a.out = ctx;
   a.ldq = ldq;
