@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "fz_internal.h"
@@ -77,7 +78,8 @@ KvQ8Batch device_view(const fz_kvq8_seqs* s) {
     need(s->starts || s->n_rows >= (uint64_t)s->n_seqs * s->max_new, "%u rows for %u sequences of %u", s->n_rows,
          s->n_seqs, s->max_new);
   }
-  return KvQ8Batch{s->pages, s->lens, s->starts, s->n_seqs, s->max_pages, s->max_new, s->n_rows, 0};
+  // no sequence has more rows than there are
+  return KvQ8Batch{s->pages, s->lens, s->starts, s->n_seqs, s->max_pages, std::min(s->max_new, s->n_rows), s->n_rows, 0};
 }
 
 // Rows of `heads` heads at p, ld elements apart; true for f16.
@@ -123,7 +125,9 @@ int fz_kvq8_read_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, v
 int fz_kvq8_attend_work(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint64_t* bytes) {
   return guard([&] {
     need(bytes != nullptr, "null argument");
-    *bytes = kvq8_attend_work(device_view(kv), device_view(s));
+    const KvQ8Batch b = device_view(s);
+    const KvQ8Dev c = device_view(kv);
+    *bytes = b.n_seqs && b.n_rows ? kvq8_attend_work(c, b) : 16;
   });
 }
 
@@ -136,6 +140,7 @@ int fz_kvq8_attend_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype,
     a.b = device_view(s);
     need(std::isfinite(scale), "scale is not finite");
     if (!a.b.n_seqs || !a.b.n_rows) return;
+    need((uint64_t)a.b.n_rows * kv->n_heads <= 0x7fffffffu, "%u rows of %u heads in one call", a.b.n_rows, kv->n_heads);
     a.f16 = check_rows("q", dtype, q, ldq, kv->n_heads, a.c.hd);
     check_rows("out", dtype, out, ldo, kv->n_heads, a.c.hd);
     need(q != out, "out must not overlap q");
