@@ -74,24 +74,35 @@ __device__ __forceinline__ void kq_st(__half* p, float v) { *p = __float2half_rn
 __device__ __forceinline__ uint32_t kq_code(float x, float s) {
   return 128 + (s > 0.f ? __float2int_rn(fminf(fmaxf(__fdiv_rn(x, s), -127.f), 127.f)) : 0);
 }
-// The same for n values, in the low bytes of w.  The product with inv = 1 / s,
-// rounded to an integer by adding 1.5 * 2^23 in one operation, is off by at most
-// 1.6e-5 before the rounding for a code up to 127, so the division, several
-// times the work, is left to threads with a value near a border (and to scales
-// too small for an inverse).
+// The same for n values, in the low bytes of w, without a division for each: with
+// inv = RN(1 / s) and lo the rest of the inverse, q = RN(x inv + x lo) is within
+// an ulp of x / s, so that RN(q + r inv) with the remainder r = x - s q, which
+// is exact, is the correctly rounded quotient (Markstein's theorem).  Adding 1.5
+// * 2^23 rounds it to an integer.  Scales whose remainders would lose bits are
+// left to the division, in a loop: it seldom runs, and code that seldom runs has
+// to be fetched first.
 template <int N>
-__device__ __forceinline__ void kq_codes(const float* x, float s, float inv, uint32_t* w) {
+__device__ __forceinline__ void kq_codes(const float* x, float s, uint32_t* w) {
   constexpr float magic = 12582912.f + 128.f;
-  bool near = !(s > 0.f);
+  if (s >= 7.8886090522101181e-31f && s <= 1.2676506002282294e30f) {  // 2^-100, 2^100
+    const float inv = __frcp_rn(s), lo = __fmul_rn(__fmaf_rn(-s, inv, 1.f), inv);
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    const float y = __fmaf_rn(x[i], inv, magic), q = __fsub_rn(y, magic);
-    near |= !(fabsf(__fmaf_rn(x[i], inv, -q)) <= 0.49998f);
-    w[i] = __float_as_uint(y);
-  }
-  if (near) {
+    for (int i = 0; i < N; i++) {
+      const float q = __fmaf_rn(x[i], inv, __fmul_rn(x[i], lo));
+      w[i] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-s, q, x[i]), inv, q), magic));
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) w[i] = kq_code(x[i], s);
+    for (int i = 0; i < N; i++) w[i] = 128;
+    if (s > 0.f) {
+      float z[N];
+#pragma unroll
+      for (int i = 0; i < N; i++) z[i] = x[i];
+#pragma unroll 1
+      for (int i = 0; i < N; i++) z[i] = __uint_as_float(kq_code(z[i], s));
+#pragma unroll
+      for (int i = 0; i < N; i++) w[i] = __float_as_uint(z[i]);
+    }
   }
 }
 // The low bytes of four words.
@@ -101,6 +112,10 @@ __device__ __forceinline__ uint32_t kq_bytes(const uint32_t* w) {
 // code + 128 of an older byte under a scale that grew by 1 / ratio
 __device__ __forceinline__ uint32_t kq_recode(uint32_t byte, float ratio) {
   return 128 + __float2int_rn(__fmul_rn((float)((int)byte - 128), ratio));
+}
+
+__device__ __forceinline__ void kq_cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
 // N consecutive, aligned elements at p.
@@ -140,147 +155,199 @@ __device__ __forceinline__ void kq_ldn(const __half* p, float* x) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.  Grid (blocks a sequence can touch, nkv, n_seqs): a CTA quantizes
-// one block of one head, its first half keys, its second half values; a thread
-// takes two 16-byte pieces, so that the call's values are read once and every
-// store is a whole piece.  A key thread's pieces are the two halves of its
-// rotated pairs.  Scale: the largest magnitude of the call's values / 127, and
-// at least the block's older scale when positions before this call's are kept;
-// those take the codes of the larger scale.  Bound by the bytes of k and v: the
-// loads of a thread are all under way before the first is used.
+// Append.  Grid (CTAs of a sequence, n_seqs).  An item is one block of one head;
+// a CTA takes every gridDim.x-th of its sequence, its first half keys, its
+// second half values, a thread two 16-byte pieces (a key thread's are the two
+// halves of its rotated pairs).  Scale: the largest magnitude of the call's
+// values / 127, and at least the block's older scale when positions before this
+// call's are kept; those take the codes of the larger scale.  Bound by the bytes
+// of k and v: the rows and rotation factors of the next two items are on their
+// way to shared memory (cp.async, whole rows) while one is quantized.  Measured:
+// 8192 positions of 8 heads of 128 in f32 (88 MB) 20.4 us (4.3 TB/s; 18.6 with
+// the codes' arithmetic left out; loads straight to registers, a CTA an item,
+// 23.3), 64 sequences of one position and 4 heads 4.8 us.  Rows of shared memory
+// are 16 bytes apart in banks for the values' four positions a thread; the
+// factors' pieces are permuted instead, since they are read 32 floats a thread.
 // ---------------------------------------------------------------------------
 template <int HD, typename T>
-__global__ void __launch_bounds__(HD) k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k,
-                                                    const T* __restrict__ v, uint64_t ld, bool late) {
+struct KqApStage {
+  static constexpr uint32_t N = 16 / sizeof(T);        // elements of a piece
+  static constexpr uint32_t CH = HD / N, RC = HD / 4;  // pieces of a row, of a position's factors
+  uint4 k[KQ_BLOCK][CH + 1], v[KQ_BLOCK][CH + 1], rope[KQ_BLOCK][RC];
+  // factor piece i of position tok
+  __device__ __forceinline__ uint4& factors(uint32_t tok, uint32_t i) {
+    return rope[tok][i ^ (i >> 3 & (HD / 32 - 1)) ^ (tok * (HD / 32) & 7)];
+  }
+};
+
+constexpr uint32_t KQ_AP_STAGES = 2;
+template <int HD>
+constexpr uint32_t kq_ap_ctas() {
+  return 512 / HD;  // CTAs per SM
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(HD, kq_ap_ctas<HD>())
+    k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k, const T* __restrict__ v, uint64_t ld, bool late) {
+  using Stage = KqApStage<HD, T>;
+  constexpr uint32_t CH = Stage::CH, RC = Stage::RC, N = Stage::N;
+  extern __shared__ uint4 kq_dyn[];
+  Stage* stages = reinterpret_cast<Stage*>(kq_dyn);
+  __shared__ uint32_t s_top[2][HD / 32];
   if (!late) pdl_trigger();
   pdl_wait();
   if (late) pdl_trigger();  // what comes next may read what this kernel's predecessors wrote before it waits
-  const KqSeq s = kq_seq(b, blockIdx.z, c.status);
-  const int32_t p0 = s.len - s.n_new;
-  const int32_t blk = p0 / (int32_t)KQ_BLOCK + (int32_t)blockIdx.x, base = blk * (int32_t)KQ_BLOCK;
-  if (s.n_new == 0 || base >= s.len) return;
+  const KqSeq s = kq_seq(b, blockIdx.y, c.status);
+  if (s.n_new == 0) return;
   if (c.rope && s.len > (int64_t)c.n_rope) {
     if (threadIdx.x == 0) atomicOr(c.status, KQ_BAD_POS);
     return;
   }
-  const int64_t entry = kq_entry(b, blockIdx.z, blk / KQ_NB);  // looked at once the values are on their way
   constexpr uint32_t U = HD / 2, half = HD / 2;  // threads of a side
-  const uint32_t h = blockIdx.y, side = threadIdx.x / U, u = threadIdx.x % U;
-  const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);  // new positions [a, e)
-  // this head's element (position base, 0)
-  const uint64_t first = (uint64_t)(s.row0 + base - p0) * ld + (uint64_t)h * HD;
-  // keys: position tok, dims d .. d + 15 and half + d ..; values: positions tok[k] = 2t, 2t + 1, 8 + 2t, 9 + 2t of dims
+  const int32_t p0 = s.len - s.n_new, last = (s.len - 1) / (int32_t)KQ_BLOCK;
+  struct Item {
+    int32_t blk;
+    uint32_t h;
+  };
+  const uint32_t dblk = gridDim.x / c.nkv, dh = gridDim.x % c.nkv;
+  const auto after = [&](const Item& i) {
+    const bool carry = i.h + dh >= c.nkv;
+    return Item{i.blk + (int32_t)(dblk + carry), i.h + dh - (carry ? c.nkv : 0)};
+  };
+  const auto issue = [&](const Item& i, Stage& st) {
+    if (i.blk <= last) {
+      const int32_t base = i.blk * (int32_t)KQ_BLOCK;
+      const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);
+      const int32_t y0 = threadIdx.x / CH, r0 = threadIdx.x / RC;
+      // elements from this head's (position base, 0), which is in the buffer for positions [a, e) only
+      const int64_t from = ((int64_t)s.row0 + base - p0 + y0) * (int64_t)ld + (int64_t)(i.h * HD + threadIdx.x % CH * N);
+#pragma unroll
+      for (uint32_t n = 0; n < KQ_BLOCK * CH / HD; n++) {
+        const int32_t y = y0 + n * (HD / CH);
+        if (y >= a && y < e) {
+          const int64_t at = from + (int64_t)(n * (HD / CH)) * (int64_t)ld;
+          kq_cp16(&st.k[y][threadIdx.x % CH], k + at);
+          kq_cp16(&st.v[y][threadIdx.x % CH], v + at);
+        }
+      }
+      if (c.rope) {
+        const auto* f = c.rope + (int64_t)(base + r0) * half + threadIdx.x % RC * 2;
+#pragma unroll
+        for (uint32_t n = 0; n < KQ_BLOCK * RC / HD; n++) {
+          const int32_t y = r0 + n * (HD / RC);
+          if (y >= a && y < e) kq_cp16(&st.factors(y, threadIdx.x % RC), f + n * (HD / RC) * half);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const uint32_t side = threadIdx.x / U, u = threadIdx.x % U;
+  // keys: position tok, dims d .. d + 15 and half + d ..; values: positions 2t, 2t + 1, 8 + 2t, 9 + 2t of dims
   // 32 q + 8 i + g and HD / 2 + that
   const uint32_t tok = u / (HD / 32), d = u % (HD / 32) * 16, g = u >> 2 & 7, t = u & 3, q = u >> 5;
-  float x[32];
+  const auto entry_of = [&](const Item& i) { return i.blk <= last ? kq_entry(b, blockIdx.y, i.blk / KQ_NB) : 0; };
+  Item now{p0 / (int32_t)KQ_BLOCK + (int32_t)(blockIdx.x / c.nkv), blockIdx.x % c.nkv}, next = after(now);
+  int64_t entry = entry_of(now);
+  issue(now, stages[0]);
+  issue(next, stages[1]);
+  uint32_t turn = 0;
+#pragma unroll 1
+  for (; now.blk <= last; turn ^= 1) {
+    const int32_t blk = now.blk, base = blk * (int32_t)KQ_BLOCK;
+    const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);  // new positions [a, e)
+    const int32_t page = kq_checked(c, entry);
+    const uint64_t at = ((uint64_t)max(page, 0) * c.nkv + now.h) * 2 + side;
+    uint8_t* codes = c.codes + at * KQ_PAGE * HD + blk % KQ_NB * KQ_BLOCK * HD;
+    float* sc = c.scales + at * KQ_NB + blk % KQ_NB;
+    const bool old = a > 0 && page >= 0;  // positions before the call's are kept
+    const float before = old ? *sc : 0.f;
+    // this thread's pieces: keys in (tile of 8 positions, 64 dims), values in (tile of 32 dims)
+    uint8_t* dst = codes + (side ? q * 512 + g * 64 + t * 16 : kq_koff<HD>(tok, d));
+    const uint32_t step = side ? HD / 64 * 512 : kq_koff<HD>(0, half);
+    uint4 kept[2];
+    if (old) kept[0] = *reinterpret_cast<const uint4*>(dst), kept[1] = *reinterpret_cast<const uint4*>(dst + step);
+    asm volatile("cp.async.wait_group %0;" ::"n"(KQ_AP_STAGES - 1) : "memory");
+    __syncthreads();
+    Stage& st = stages[turn];
+    float x[32];
 #pragma unroll
-  for (int i = 0; i < 32; i++) x[i] = 0.f;
-  if (side == 0) {
-    if ((int32_t)tok >= a && (int32_t)tok < e) {
-      const T* p = k + first + (uint64_t)tok * ld + d;
-      kq_ldn<16>(p, x);
-      kq_ldn<16>(p + half, x + 16);
-      if (c.rope) {
-        float f[32];
-        kq_ldn<32>(reinterpret_cast<const float*>(c.rope + (uint64_t)(base + tok) * half + d), f);
+    for (int i = 0; i < 32; i++) x[i] = 0.f;
+    if (side == 0) {
+      if ((int32_t)tok >= a && (int32_t)tok < e) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float m = x[i], w = x[16 + i];
-          x[i] = __fsub_rn(__fmul_rn(m, f[2 * i]), __fmul_rn(w, f[2 * i + 1]));
-          x[16 + i] = __fadd_rn(__fmul_rn(m, f[2 * i + 1]), __fmul_rn(w, f[2 * i]));
+        for (uint32_t i = 0; i < 16 / N; i++) {
+          kq_ldn<N>(reinterpret_cast<const T*>(&st.k[tok][d / N + i]), x + i * N);
+          kq_ldn<N>(reinterpret_cast<const T*>(&st.k[tok][CH / 2 + d / N + i]), x + 16 + i * N);
         }
-      }
-    }
-  } else {
+        if (c.rope) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int32_t y = (j >> 1) * 8 + 2 * t + (j & 1);
-      if (y >= a && y < e) {
-        const T* p = v + first + (uint64_t)y * ld + 32 * q + g;
+          for (uint32_t i = 0; i < 8; i++) {
+            const uint4 w = st.factors(tok, d / 2 + i);
+            const float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)};
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[4 * i + j] = kq_ld(p + (i >> 2) * half + (i & 3) * 8);
-      }
-    }
-  }
-  const int32_t page = kq_checked(c, entry);
-  if (page < 0) return;
-  const uint64_t at = ((uint64_t)page * c.nkv + h) * 2 + side;
-  uint8_t* codes = c.codes + at * KQ_PAGE * HD + blk % KQ_NB * KQ_BLOCK * HD;
-  float* sc = c.scales + at * KQ_NB + blk % KQ_NB;
-  const float before = a > 0 ? *sc : 0.f;
-  uint4 kept[2];  // value pieces that hold older positions
-  if (side && a > 0) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-      kept[i] = *reinterpret_cast<const uint4*>(codes + (q + i * (HD / 64)) * 512 + g * 64 + t * 16);
-  }
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 32; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[i])));
-  if (!(top <= 3.402823466e38f)) {
-    atomicOr(c.status, KQ_NOT_FINITE);
-    top = INFINITY;
-  }
-  // largest magnitude of the side; non-negative floats order like their bits, and a side with a value that is not
-  // finite ends with infinity
-  __shared__ uint32_t s_top[2];
-  if (threadIdx.x < 2) s_top[threadIdx.x] = 0;
-  __syncthreads();
-  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-  if ((threadIdx.x & 31) == 0) atomicMax(&s_top[side], bits);
-  __syncthreads();
-  top = __uint_as_float(s_top[side]);
-  float scale = __fdiv_rn(top, 127.f);
-  if (a > 0 && !(scale > before)) scale = before;
-  if (top == INFINITY) scale = __int_as_float(0x7fffffff);  // no number, not a wrong one
-  const bool grew = a > 0 && scale > before;
-  const float ratio = __fdiv_rn(before, scale), inv = __fdiv_rn(1.f, scale);
-  if (u == 0) *sc = scale;
-  if (side == 0) {
-    uint4* dst[2] = {reinterpret_cast<uint4*>(codes + kq_koff<HD>(tok, d)),
-                     reinterpret_cast<uint4*>(codes + kq_koff<HD>(tok, half + d))};
-    if ((int32_t)tok >= e || ((int32_t)tok < a && !grew)) return;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      uint32_t w[4];
-      if ((int32_t)tok < a) {
-        const uint4 old = *dst[i];
-        const uint32_t o[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-          w[m] = 0;
-#pragma unroll
-          for (int n = 0; n < 4; n++) w[m] |= kq_recode(o[m] >> (8 * n) & 255, ratio) << (8 * n);
-        }
-      } else {
-        uint32_t y[16];
-        kq_codes<16>(x + 16 * i, scale, inv, y);
-#pragma unroll
-        for (int m = 0; m < 4; m++) w[m] = kq_bytes(y + 4 * m);
-      }
-      *dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      uint4* dst = reinterpret_cast<uint4*>(codes + (q + i * (HD / 64)) * 512 + g * 64 + t * 16);
-      uint32_t w[4], y[16];
-      kq_codes<16>(x + 16 * i, scale, inv, y);
-#pragma unroll
-      for (int m = 0; m < 4; m++) w[m] = kq_bytes(y + 4 * m);
-      if (a > 0) {  // positions before the call's are kept
-        const uint32_t o[4] = {kept[i].x, kept[i].y, kept[i].z, kept[i].w};
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-#pragma unroll
-          for (int n = 0; n < 4; n++) {
-            if ((n >> 1) * 8 + 2 * (int32_t)t + (n & 1) >= a) continue;
-            const uint32_t byte = o[m] >> (8 * n) & 255;
-            w[m] = (w[m] & ~(255u << (8 * n))) | (grew ? kq_recode(byte, ratio) : byte) << (8 * n);
+            for (uint32_t n = 0; n < 2; n++) {
+              const float m = x[2 * i + n], o = x[16 + 2 * i + n];
+              x[2 * i + n] = __fsub_rn(__fmul_rn(m, f[2 * n]), __fmul_rn(o, f[2 * n + 1]));
+              x[16 + 2 * i + n] = __fadd_rn(__fmul_rn(m, f[2 * n + 1]), __fmul_rn(o, f[2 * n]));
+            }
           }
+        }
       }
-      *dst = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int32_t j = 0; j < 4; j++) {
+        const int32_t y = (j >> 1) * 8 + 2 * t + (j & 1);
+        if (y >= a && y < e) {
+          const T* p = reinterpret_cast<const T*>(st.v[y]) + 32 * q + g;
+#pragma unroll
+          for (uint32_t i = 0; i < 8; i++) x[4 * i + j] = kq_ld(p + (i >> 2) * half + (i & 3) * 8);
+        }
+      }
     }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(x[i]), "f"(x[i + 1]));
+    if (!(top <= 3.402823466e38f)) {
+      if (page >= 0) atomicOr(c.status, KQ_NOT_FINITE);
+      top = INFINITY;
+    }
+    // largest magnitude of the side; non-negative floats order like their bits, and a side with a value that is not
+    // finite ends with infinity
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if ((threadIdx.x & 31) == 0) s_top[turn][threadIdx.x >> 5] = bits;
+    __syncthreads();  // the stage's rows are read, too
+    now = next;
+    next = after(next);
+    issue(next, st);
+    entry = entry_of(now);
+    if (page < 0) continue;
+    top = __uint_as_float(s_top[turn][side * (HD / 64)]);
+    if (HD == 128) top = fmaxf(top, __uint_as_float(s_top[turn][side * 2 + 1]));
+    float scale = __fdiv_rn(top, 127.f);
+    if (a > 0 && !(scale > before)) scale = before;
+    if (top == INFINITY) scale = __int_as_float(0x7fffffff);  // no number, not a wrong one
+    const bool grew = a > 0 && scale > before;
+    if (u == 0) *sc = scale;
+    uint32_t w[32];
+    kq_codes<32>(x, scale, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = kq_bytes(w + 4 * i);
+    if (a > 0) {
+      const float ratio = __fdiv_rn(before, scale);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint32_t o = reinterpret_cast<const uint32_t*>(kept)[i];
+#pragma unroll
+        for (int32_t n = 0; n < 4; n++) {
+          if ((side ? (n >> 1) * 8 + 2 * (int32_t)t + (n & 1) : (int32_t)tok) >= a) continue;
+          const uint32_t byte = o >> (8 * n) & 255;
+          w[i] = (w[i] & ~(255u << (8 * n))) | (grew ? kq_recode(byte, ratio) : byte) << (8 * n);
+        }
+      }
+    }
+    if (side == 0 && (int32_t)tok >= e) continue;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + step) = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
@@ -458,9 +525,6 @@ __device__ __forceinline__ void kq_split2(float a, float b, uint32_t* hi, uint32
   const float2 f = __half22float2(h);
   *hi = *reinterpret_cast<const uint32_t*>(&h);
   *lo = kq_pack((a - f.x) * 2048.f, (b - f.y) * 2048.f);
-}
-__device__ __forceinline__ void kq_cp16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void kq_cp8(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -1594,15 +1658,36 @@ __global__ void __launch_bounds__(KR_JOIN_THREADS) k_kvq8_join(const __grid_cons
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
+// Runs f once for each device (a kernel's attributes hold per device); devices
+// past the 64 bits run it every time.
+template <class F>
+static void kvq8_once(std::atomic<uint64_t>& ready, F&& f) {
+  int dev = 0;
+  CK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (ready.load(std::memory_order_acquire) & bit) return;
+  f();
+  ready.fetch_or(bit, std::memory_order_release);
+}
+
 // Blocks that max_new consecutive positions can touch.
 static uint32_t kvq8_blocks(const KvQ8Batch& b) { return (b.max_new + 2 * KQ_BLOCK - 2) / KQ_BLOCK; }
 
 template <int HD, typename T>
 static void kvq8_append_t(const KvQ8Dev& c, const KvQ8Batch& b, const void* k, const void* v, uint64_t ld, bool late,
                           cudaStream_t s) {
-  const dim3 grid(kvq8_blocks(b), c.nkv, b.n_seqs);
-  launch_pdl(k_kvq8_append<HD, T>, grid, dim3(HD), 0, s, c, b, static_cast<const T*>(k),
-             static_cast<const T*>(v), ld, late);
+  using Stages = KqApStage<HD, T>[KQ_AP_STAGES];
+  static std::atomic<uint64_t> ready{0};
+  kvq8_once(ready, [&] {
+    CK(cudaFuncSetAttribute(k_kvq8_append<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Stages)));
+  });
+  // one sequence: every SM filled once, a CTA taking as many items as that leaves it (8192 positions of 8 heads 20.4 us;
+  // an item a CTA 23.0).  Several may be shorter than max_new: an item a CTA keeps the SMs even (ragged prompts 7 us;
+  // cut like one sequence 10)
+  const uint64_t items = (uint64_t)kvq8_blocks(b) * c.nkv, slots = (uint64_t)num_sms() * kq_ap_ctas<HD>();
+  const uint64_t per = b.n_seqs > 1 ? 1 : (items + slots - 1) / slots;
+  launch_pdl(k_kvq8_append<HD, T>, dim3((unsigned)((items + per - 1) / per), b.n_seqs), dim3(HD), sizeof(Stages), s, c,
+             b, static_cast<const T*>(k), static_cast<const T*>(v), ld, late);
 }
 
 void launch_kvq8_append(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, const void* k, const void* v, uint64_t ld,
@@ -1626,18 +1711,6 @@ void launch_kvq8_read(const KvQ8Dev& c, const KvQ8Batch& b, bool f16, void* k, v
     f16 ? kvq8_read_t<128, __half>(c, b, k, v, ld, s) : kvq8_read_t<128, float>(c, b, k, v, ld, s);
   else
     f16 ? kvq8_read_t<64, __half>(c, b, k, v, ld, s) : kvq8_read_t<64, float>(c, b, k, v, ld, s);
-}
-
-// Runs f once for each device (a kernel's attributes hold per device); devices
-// past the 64 bits run it every time.
-template <class F>
-static void kvq8_once(std::atomic<uint64_t>& ready, F&& f) {
-  int dev = 0;
-  CK(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (ready.load(std::memory_order_acquire) & bit) return;
-  f();
-  ready.fetch_or(bit, std::memory_order_release);
 }
 
 // Runs of the split form: every SM filled, never more than there can be tiles.

@@ -181,3 +181,29 @@ def test_rows_of_a_fused_projection(gpu):
         for j in (0, new // 2, new - 1):
             want, tol = d.plain.attend(t[0], end - new + j + 1, x[j:j + 1, :8])
             assert (np.abs(got[j, 64:576].reshape(1, 8, 64) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_codes_at_rounding_borders(gpu, hd):
+    """Values a few units in the last place around half codes, for scales of
+    every magnitude (smallest 2^-140, largest 2^120): the codes are those of a
+    rounded f32 division, bit for bit."""
+    n = 16 * 44
+    d = Dev((n + PAGE - 1) // PAGE, 2, 2, hd)
+    t = d.table([n])
+    shape = (44, 16, 2, hd)
+    exps = np.linspace(-140, 120, 44).astype(int)
+    both = []
+    for _ in range(2):
+        top = (np.ldexp(d.rng.uniform(1, 2, (44, 1, 2, 1)), exps[:, None, None, None]) * 63.5).astype(np.float32)
+        scale = top / np.float32(127)
+        x = ((d.rng.integers(-127, 127, shape) + 0.5).astype(np.float32) * scale).astype(np.float32)
+        x = (x.view(np.int32) + d.rng.integers(-3, 4, shape).astype(np.int32)).view(np.float32)
+        x = np.clip(np.where(np.isfinite(x), x, np.float32(0)), -top, top)
+        x[:, 0, :, 0] = top[:, 0, :, 0]
+        x = x.reshape(n, 2, hd)
+        both.append((x, gpu.from_numpy(x.reshape(n, -1)).cuda()))
+    d.append(t, [n], [n], k=both[0], v=both[1])
+    gpu.cuda.synchronize()
+    d.check_cache([(t[0], n)])
+    d.c.status(d.stream())
