@@ -344,8 +344,9 @@ enum { FZ_KVQ8_PAGE = 64, FZ_KVQ8_BLOCK = 16 };
  *           + (p / 8) * 2 + p % 2
  * scales: [n_pages][n_kv_heads][2][4] f32.  rope: [n_rope][head_dim / 2][2] f32
  * (cos, sin) of every position, or NULL with n_rope 0: keys and queries are
- * then taken as they are.  head_dim is 64 or 128; n_heads (the query heads) a
- * multiple of n_kv_heads.  Neither codes nor scales need to be initialised. */
+ * then taken as they are.  scales and rope are 16-byte aligned, too.  head_dim
+ * is 64 or 128; n_heads (the query heads) a multiple of n_kv_heads.  Neither
+ * codes nor scales need to be initialised. */
 typedef struct fz_kvq8 {
   void* codes;
   float* scales;
