@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(HD, kq_ap_ctas<HD>())
 // Read-back: the rows a batch names as values.  Grid (blocks a sequence can
 // touch, nkv, n_seqs): a CTA takes one block of one head; the pieces pass
 // through shared memory, since a value piece holds four positions of four dims.
-// Bound by the bytes: 8295 positions of 8 heads of 128 to f16 (51 MB) 11.3 us.
+// Bound by the bytes: 8192 positions of 8 heads of 128 to f16 (51 MB) 11.3 us.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void kq_st4(float* p, const float* x) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
