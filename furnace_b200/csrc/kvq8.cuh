@@ -118,6 +118,24 @@ __device__ __forceinline__ void kq_cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
+// a * b + c of two pairs in one instruction, each rounded by itself.
+__device__ __forceinline__ float2 kq_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 kq_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // N consecutive, aligned elements at p.
 template <int N>
 __device__ __forceinline__ void kq_ldn(const float* p, float* x) {
@@ -445,9 +463,9 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // Measured with the merge: 16 sequences of 32768 positions, 8 KV heads of 128,
 // 64 query heads (1.08 GB) 188 us, 5.7 TB/s (226 us where calls follow each
 // other for seconds: the power limit); 48 ragged ones of up to 8192, 4 KV heads
-// (208 MB) 50 us, of which about 5 pass before the first page has come and 3 in
-// the merge.  16 rows a segment, or more runs than the SMs hold at once, are not
-// faster.
+// (208 MB) 49 us, of which about 5 pass before the first page has come and 3 in
+// the merge.  Multiplies and sums in pairs took the last 2 %.  16 rows a segment,
+// or more runs than the SMs hold at once, are not faster.
 // ---------------------------------------------------------------------------
 constexpr int KQ_SP_THREADS = 128;
 constexpr uint32_t KQ_SP_STAGES = 2;     // tiles of a warp in shared memory
@@ -532,7 +550,8 @@ __device__ __forceinline__ void kq_split2(float a, float b, uint32_t* hi, uint32
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
   *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = kq_pack((a - f.x) * 2048.f, (b - f.y) * 2048.f);
+  const float2 r = kq_fma2(f, make_float2(-2048.f, -2048.f), make_float2(a * 2048.f, b * 2048.f));
+  *lo = kq_pack(r.x, r.y);
 }
 __device__ __forceinline__ void kq_cp8(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -783,8 +802,10 @@ __device__ __forceinline__ void kq_segment(const KqSplitArgs<HD, T>& a, KqSplitS
           kq_mma(d, pa[0], h[0], h[1]);
           kq_halves(word[4 + k], h);
           kq_mma(d, pa[1], h[0], h[1]);
-          o[n * 4 + k][0] += fmaf(d[2], 1.f / 2048.f, d[0]);
-          o[n * 4 + k][1] += fmaf(d[3], 1.f / 2048.f, d[1]);
+          const float2 sum = kq_fma2(make_float2(d[2], d[3]), make_float2(1.f / 2048.f, 1.f / 2048.f),
+                                     make_float2(d[0], d[1]));
+          const float2 y = kq_add2(make_float2(o[n * 4 + k][0], o[n * 4 + k][1]), sum);
+          o[n * 4 + k][0] = y.x, o[n * 4 + k][1] = y.y;
         }
       }
     }
@@ -1156,24 +1177,6 @@ struct KrPages {
   __device__ __forceinline__ uint32_t at(uint32_t n) const { return __shfl_sync(0xffffffffu, cur, n % 32); }
 };
 
-// a * b + c of two pairs in one instruction, each rounded by itself.
-__device__ __forceinline__ float2 kr_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 kr_add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // One row and 16 positions (a block) of a step.  f and lv are the block's score
 // factor and the log2 of its value scale, bits the positions that the row sees
 // (MASK).
@@ -1195,7 +1198,7 @@ __device__ __forceinline__ void kr_put(const float* x, uint32_t t) {
     const __half2 h = __floats2half2_rn(a, z);
     const float2 g = __half22float2(h);
     hi[c] = *reinterpret_cast<const uint32_t*>(&h);
-    const float2 r = kr_fma2(g, make_float2(-1.f, -1.f), make_float2(a, z));
+    const float2 r = kq_fma2(g, make_float2(-1.f, -1.f), make_float2(a, z));
     lo[c] = kq_pack(r.x, r.y);
   }
   kr_st8(t, hi);
@@ -1207,10 +1210,10 @@ __device__ __forceinline__ float kr_weights(float* x, float f, float c) {
   float2 sum[2] = {};
 #pragma unroll
   for (int k = 0; k < 16; k += 2) {
-    const float2 e = kr_fma2(make_float2(x[k], x[k + 1]), make_float2(f, f), make_float2(c, c));
+    const float2 e = kq_fma2(make_float2(x[k], x[k + 1]), make_float2(f, f), make_float2(c, c));
     x[k] = kq_exp2(e.x);
     x[k + 1] = kq_exp2(e.y);
-    sum[k / 2 & 1] = kr_add2(sum[k / 2 & 1], make_float2(x[k], x[k + 1]));
+    sum[k / 2 & 1] = kq_add2(sum[k / 2 & 1], make_float2(x[k], x[k + 1]));
   }
   return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
