@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // finite.
 //
 // Measured with the merge: 16 sequences of 32768 positions, 8 KV heads of 128,
-// 64 query heads (1.08 GB) 188 us, 5.7 TB/s (226 us where calls follow each
+// 64 query heads (1.08 GB) 188 us, 5.7 TB/s (220 us where calls follow each
 // other for seconds: the power limit); 48 ragged ones of up to 8192, 4 KV heads
 // (208 MB) 49 us, of which about 5 pass before the first page has come and 3 in
 // the merge.  Multiplies and sums in pairs took the last 2 %.  16 rows a segment,
