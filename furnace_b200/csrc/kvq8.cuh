@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(HD, kq_ap_ctas<HD>())
       const int32_t a = max(p0 - base, 0), e = min(s.len - base, (int32_t)KQ_BLOCK);
       const int32_t y0 = threadIdx.x / CH, r0 = threadIdx.x / RC;
       // elements from this head's (position base, 0), which is in the buffer for positions [a, e) only
-      const int64_t from = ((int64_t)s.row0 + base - p0 + y0) * (int64_t)ld + (int64_t)(i.h * HD + threadIdx.x % CH * N);
+      const int64_t from =
+          ((int64_t)s.row0 + base - p0 + y0) * (int64_t)ld + (int64_t)(i.h * HD + threadIdx.x % CH * N);
 #pragma unroll
       for (uint32_t n = 0; n < KQ_BLOCK * CH / HD; n++) {
         const int32_t y = y0 + n * (HD / CH);
@@ -1432,8 +1433,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     };
     load(ids.at(0), w[0]);
     load(ids.at(1), w[1]);
-    // the rows first: both share the issue slots, and the values are not needed before the first weights (105.4 -> 104.2
-    // us for 2048 rows)
+    // the rows first: both share the issue slots, and the values are not needed before the first weights (105.4 ->
+    // 104.2 us for 2048 rows)
     ok = __all_sync(0xffffffffu, mbar_wait(&sm.q_full, 0));
     values(0);
     float acc[HD];
