@@ -207,3 +207,23 @@ def test_codes_at_rounding_borders(gpu, hd):
     gpu.cuda.synchronize()
     d.check_cache([(t[0], n)])
     d.c.status(d.stream())
+
+
+@pytest.mark.parametrize("hd, kv, dtype", [(64, 16, fz.F16), (128, 8, fz.F32), (128, 7, fz.F16), (64, 9, fz.F32)])
+def test_append_of_more_blocks_than_fit_at_once(gpu, hd, kv, dtype):
+    """One sequence, so many blocks and heads that a CTA takes several of them,
+    entered in the middle of a block; what is read back is what was written."""
+    end = 3701
+    d = Dev((end + PAGE - 1) // PAGE, kv, kv, hd, end)
+    t = d.table([end])
+    d.append(t, [37], [37], dtype)
+    d.append(t, [end], [end - 37], dtype, k=d.rows(end - 37, kv, dtype, spread=3.0))
+    gpu.cuda.synchronize()
+    d.check_cache([(t[0], end)])
+    s = d.seqs(t, [end], [end])
+    k, v = (gpu.full((end, kv * hd), 9.0, device="cuda") for _ in range(2))
+    d.c.read(s, k.data_ptr(), v.data_ptr(), kv * hd, stream=d.stream())
+    gpu.cuda.synchronize()
+    for got, want in zip((k, v), d.plain.rows(t[0], 0, end, np.float32)):
+        assert np.array_equal(got.cpu().numpy().reshape(end, kv, hd).transpose(1, 0, 2), want)
+    d.c.status(d.stream())
