@@ -1296,7 +1296,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
   // With n buffers, step i uses buffer i % n, for the (i / n)th time: a wait for
   // step i's use is a wait for parity (i / n) % 2.  No barrier may get a whole
   // use ahead of a thread that still waits for the one before; beside each wait
-  // stands what the next use needs from that thread.
+  // stands what the next use needs from that thread.  A wait that runs out does
+  // so by each lane's own clock: where a warp goes on together, its lanes agree
+  // (__all_sync) before what needs them all.
   auto wait = [&](auto& bar, uint32_t i) {
     constexpr uint32_t n = sizeof(bar) / sizeof(uint64_t);
     return mbar_wait(reinterpret_cast<uint64_t*>(&bar) + i % n, (i / n) & 1);
@@ -1343,7 +1345,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
         umma_commit(&sm.o_full);
       }
       umma_commit(&sm.fin);  // everything issued, whether or not a wait ran out
-      mbar_wait(&sm.fin, 0);
+      ok = mbar_wait(&sm.fin, 0) && ok;
     }
     __syncwarp();
   } else if (warp >= 12) {
@@ -1458,7 +1460,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       tc_fence_before();
       mbar_arrive(&sm.o_free);
     }
-    ok = ok && mbar_wait(&sm.l_full, 0);
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.l_full, 0));
     // The result goes out through shared memory (the operands': every product is done), a warp a row at a time.  Each
     // warpgroup's denominator goes by the maximum of its own last step, the sums by that of the last.
     if (ok) {

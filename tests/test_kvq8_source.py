@@ -1,0 +1,53 @@
+"""Rules of the prompt kernel (k_kvq8_rows) that no run can show: a wait that
+runs out does so by each lane's own clock, and making one run out on a GPU
+would need a broken kernel.  So its source is read."""
+
+import os
+import re
+
+import furnace_b200 as fz
+
+KVQ8 = os.path.join(os.path.dirname(fz.__file__), "csrc", "kvq8.cuh")
+
+
+def _code():
+    with open(KVQ8) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+def _rows_kernel():
+    code = _code()
+    body = code[code.index("k_kvq8_rows(const __grid_constant__"):]
+    return body[:body.index("\n}\n")]
+
+
+def _statements(code):
+    """Statements that wait on a barrier (the helper's own definition aside)."""
+    out = []
+    for s in re.split(r"[;{}]", code):
+        if re.search(r"\b(mbar_wait|wait)\(", s) and "auto wait" not in s and "reinterpret_cast" not in s:
+            out.append(" ".join(s.split()))
+    return out
+
+
+def test_every_wait_of_a_warp_ends_for_all_its_lanes_alike():
+    """What follows a wait uses the whole warp (tensor memory loads, shuffles,
+    __syncwarp), so lanes of a warp must never come to different ends: the
+    result goes through __all_sync.  The one thread that issues the products is
+    alone, and each of its waits decides what it does next."""
+    body = _rows_kernel()
+    lo = body.index("if (warp == 15) {\n    if (lane == 0) {")
+    hi = body.index("} else if (warp >= 12) {")
+    alone, warps = _statements(body[lo:hi]), _statements(body[:lo] + body[hi:])
+    assert len(alone) >= 5 and len(warps) >= 6
+    for s in warps:
+        assert "__all_sync(0xffffffffu," in s, s
+        assert re.match(r"(if \(.*\) )?(bool )?ok = ", s), s
+    for s in alone:
+        assert re.search(r"\bok = ", s), s
+
+
+def test_a_wait_that_ran_out_is_reported():
+    body = _rows_kernel()
+    end = body[body.rindex("__syncthreads()") - 200:]
+    assert "if (!ok && lane == 0) atomicOr(a.c.status, KQ_TIMEOUT)" in end
