@@ -13,6 +13,12 @@
 //   keys    [8 positions][64 dims] tiles: piece (position g, dims 16t..16t+15)
 //   values  [32 dims] tiles: piece (g, t) = 4 words i, the word's bytes being
 //           positions 2t, 2t + 1, 8 + 2t, 9 + 2t of dim 8i + g
+//
+// What a kernel reads, the kernel before it may still be writing while this one
+// is resident and waits (programmatic dependent launch).  So nothing here goes
+// through the read-only path (ld.global.nc, which the compiler may also take for
+// const __restrict__ pointers): that is for memory that stays the same for a
+// kernel's whole life.
 constexpr uint32_t KQ_PAGE = 64;   // positions of a page
 constexpr uint32_t KQ_BLOCK = 16;  // positions that share a scale
 constexpr uint32_t KQ_NB = KQ_PAGE / KQ_BLOCK;
@@ -206,7 +212,7 @@ constexpr uint32_t kq_ap_ctas() {
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(HD, kq_ap_ctas<HD>())
-    k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* __restrict__ k, const T* __restrict__ v, uint64_t ld, bool late) {
+    k_kvq8_append(KvQ8Dev c, KvQ8Batch b, const T* k, const T* v, uint64_t ld, bool late) {
   using Stage = KqApStage<HD, T>;
   constexpr uint32_t CH = Stage::CH, RC = Stage::RC, N = Stage::N;
   extern __shared__ uint4 kq_dyn[];
@@ -1057,7 +1063,8 @@ __global__ void __launch_bounds__(KQ_MG_THREADS) k_kvq8_merge(const __grid_const
 // k_kvq8_join joins.
 //
 // Measured: 2048 rows of 28 heads behind 100 positions, 4 KV heads of 128, f32,
-// 104 us (33 GFLOP, done twice for the two parts: 0.63 PFLOP/s).  A step takes
+// 105 us (33 GFLOP, done twice for the two parts: 0.62 PFLOP/s; 104 with the keys
+// through the read-only path, which is not theirs to take).  A step takes
 // about 3800 cycles, 1300 of them the products': the softmax's and the
 // conversions' instructions bound it (multiplies and sums in pairs gave 2 %).  A
 // CTA's start and end take 27K of its 60K cycles on average: 10K until the rows
@@ -1361,7 +1368,7 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       for (uint32_t x = 0; x < X; x++) {
         const uint32_t tile = cw + KR_CONV * x;
         if (tile < NT)
-          w[x] = __ldg(reinterpret_cast<const uint4*>(src + (tile < NT / 2 ? pa : pb) * stride + tile % (NT / 2) * 512));
+          w[x] = *reinterpret_cast<const uint4*>(src + (tile < NT / 2 ? pa : pb) * stride + tile % (NT / 2) * 512);
       }
     };
     KrPages ids(page_of, lane);
@@ -1403,8 +1410,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
                            g * 64 + (lane >> 3 & 1) * 32;
 #pragma unroll
       for (uint32_t x = 0; x < X; x++) {
-        v[2 * x] = __ldg(reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024));
-        v[2 * x + 1] = __ldg(reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024 + 16));
+        v[2 * x] = *reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024);
+        v[2 * x + 1] = *reinterpret_cast<const uint4*>(src + (cw + 4 * x) * 1024 + 16);
       }
     };
     KrPages ids(page_of, lane);
@@ -1572,8 +1579,8 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     // a step's scales, one block a lane (lanes 0-7 and their likes), loaded two steps ahead
     auto scales = [&](uint32_t page, float* ks, float* vs) {
       const float* p = a.c.scales + ((uint64_t)page * a.c.nkv + kvh) * 2 * KQ_NB + (lane & 3);
-      *ks = __ldg(p);
-      *vs = __ldg(p + KQ_NB);
+      *ks = p[0];
+      *vs = p[KQ_NB];
     };
     float ks_next, vs_next;
     scales(page_of(2 * wg + side), &ks_next, &vs_next);

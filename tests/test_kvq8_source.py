@@ -1,6 +1,7 @@
-"""Rules of the prompt kernel (k_kvq8_rows) that no run can show: a wait that
-runs out does so by each lane's own clock, and making one run out on a GPU
-would need a broken kernel.  So its source is read."""
+"""Rules of the 8-bit cache's kernels that no run can show: a wait that runs out
+does so by each lane's own clock, and making one run out on a GPU would need a
+broken kernel; a load through the read-only path sees old bytes once in a long
+while or never.  So the source is read."""
 
 import os
 import re
@@ -51,3 +52,11 @@ def test_a_wait_that_ran_out_is_reported():
     body = _rows_kernel()
     end = body[body.rindex("__syncthreads()") - 200:]
     assert "if (!ok && lane == 0) atomicOr(a.c.status, KQ_TIMEOUT)" in end
+
+
+def test_nothing_is_read_through_the_read_only_path():
+    """The kernel before may still be writing the cache, the rows and the
+    lengths while these kernels are resident."""
+    code = _code()
+    assert "__ldg" not in code and ".nc" not in code
+    assert not re.search(r"const [\w:]+\s*\*\s*__restrict__", code)
