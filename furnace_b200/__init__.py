@@ -487,8 +487,8 @@ KVQ8_PAGE, KVQ8_BLOCK = 64, 16  # positions of a page, positions that share a sc
 class KvQ8Seqs:
     """The sequences of a call (fz_kvq8_seqs): device addresses of the page
     table [n_seqs, max_pages], the lengths [n_seqs] and, unless every sequence
-    has max_new rows, the row starts [n_seqs + 1], all int32.  The caller keeps
-    the buffers alive."""
+    has max_new rows (one of length 0 none), the row starts [n_seqs + 1], all
+    int32.  The caller keeps the buffers alive."""
 
     def __init__(self, pages: int, lens: int, n_seqs: int, max_pages: int, n_rows: int, starts: int | None = None,
                  max_new: int = 1):

@@ -42,6 +42,8 @@ __device__ __forceinline__ KqSeq kq_seq(const KvQ8Batch& b, uint32_t i, uint32_t
   if (b.starts) {
     r0 = b.starts[i];
     n = (int64_t)b.starts[i + 1] - r0;
+  } else if (len == 0) {
+    n = 0;  // an idle slot of a batch of fixed size
   }
   if (len < 0 || len > (int64_t)b.max_pages * KQ_PAGE || n < 0 || n > b.max_new || n > len || r0 < 0 ||
       r0 + n > b.n_rows) {

@@ -361,8 +361,9 @@ typedef struct fz_kvq8 {
  * positions each sequence holds, this call's among them; 0 is a sequence
  * without positions.  starts: [n_seqs + 1], sequence i's last starts[i + 1] -
  * starts[i] (0 .. max_new) positions are rows starts[i] .. of the call's row
- * buffers; NULL: every sequence has max_new rows, i * max_new ...  n_rows: the
- * rows the buffers hold (rows of no sequence are left as they are). */
+ * buffers; NULL: every sequence has max_new rows, i * max_new .., but one of
+ * length 0 (an idle slot of a batch of fixed size) has none.  n_rows: the rows
+ * the buffers hold (rows of no sequence are left as they are). */
 typedef struct fz_kvq8_seqs {
   const int32_t* pages;
   const int32_t* lens;
