@@ -1,5 +1,6 @@
 // fz_kvq8_*: the 8-bit paged KV cache on the caller's device buffers.  Checks
-// of arguments and the choice of the device; the kernels are in kvq8.cuh.
+// of arguments, the choice of the device and the reports of the status word; the
+// operators' kernels are in kvq8.cuh.
 
 #include <cuda_runtime.h>
 
@@ -92,6 +93,27 @@ bool check_rows(const char* what, uint32_t dtype, const void* p, uint64_t ld, ui
   return dtype == FZ_F16;
 }
 
+__global__ void k_take_bits(uint32_t* word, uint32_t* found) { *found = atomicExch(word, 0u); }
+
+// Reads the word and clears it in one step: a bit that a call on another stream
+// sets meanwhile is read here or stays for the next time.
+uint32_t take_bits(uint32_t* word, cudaStream_t s) {
+  struct Scratch {
+    void* p = nullptr;
+    cudaStream_t s;
+    ~Scratch() {
+      if (p) cudaFreeAsync(p, s);
+    }
+  } found{nullptr, s};
+  uint32_t bits = 0;
+  ck(cudaMallocAsync(&found.p, 4, s), "cudaMallocAsync");
+  k_take_bits<<<1, 1, 0, s>>>(word, static_cast<uint32_t*>(found.p));
+  ck(cudaGetLastError(), "k_take_bits");
+  ck(cudaMemcpyAsync(&bits, found.p, 4, cudaMemcpyDeviceToHost, s), "cudaMemcpyAsync");
+  ck(cudaStreamSynchronize(s), "cudaStreamSynchronize");
+  return bits;
+}
+
 }  // namespace
 
 extern "C" {
@@ -169,8 +191,8 @@ int fz_kvq8_status(const fz_kvq8* kv, void* stream) {
     ck(cudaMemcpyAsync(&bits, c.status, 4, cudaMemcpyDeviceToHost, s), "cudaMemcpyAsync");
     ck(cudaStreamSynchronize(s), "cudaStreamSynchronize");
     if (!bits) return;
-    ck(cudaMemsetAsync(c.status, 0, 4, s), "cudaMemsetAsync");
-    ck(cudaStreamSynchronize(s), "cudaStreamSynchronize");
+    bits = take_bits(c.status, s);
+    if (!bits) return;  // another report has them
     if (bits & KQ_TIMEOUT) fail(FZ_ETIMEOUT, "8-bit KV cache: a bounded device wait ran out");
     fail(FZ_EINVAL, "8-bit KV cache:%s%s%s%s", bits & KQ_BAD_LEN ? " lengths or rows out of range;" : "",
          bits & KQ_BAD_PAGE ? " page number out of range;" : "",

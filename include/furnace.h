@@ -405,7 +405,8 @@ int fz_kvq8_read_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, v
                      void* stream);
 
 /* Wait for `stream`, then report what the kernels found in their inputs since
- * the last report: FZ_EINVAL with a message naming it, FZ_OK if nothing. */
+ * the last report: FZ_EINVAL with a message naming it, FZ_OK if nothing.  What
+ * a call on another stream finds meanwhile is in this report or in the next. */
 int fz_kvq8_status(const fz_kvq8* kv, void* stream);
 
 #if defined(__GNUC__)

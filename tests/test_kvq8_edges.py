@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import furnace_b200 as fz
-from tests.test_kvq8 import Dev, gpu  # noqa: F401  (the module's GPU fixture)
+from tests.test_kvq8 import PAGE, Dev, gpu  # noqa: F401  (the module's GPU fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,36 @@ def test_a_uniform_sequence_shorter_than_its_rows_is_still_refused(gpu):
     d.c.attend(s, q[1].data_ptr(), out.data_ptr(), 256, 256, work.data_ptr(), work.numel(), stream=d.stream())
     with pytest.raises(fz.FurnaceError, match="lengths or rows"):
         d.c.status(d.stream())
+
+
+def test_status_keeps_what_another_stream_finds_meanwhile(gpu):
+    """A report takes the bits that it names and no others: one that a call on
+    another stream sets while a report is under way is in this report or in the
+    next.  The other stream's call is delayed by more and more, so that it meets
+    every moment of the report."""
+    d = Dev(8, 4, 2, 64, 200)
+    t = d.table([40, 90])
+    d.append(t, [40, 90], [40, 90])
+    bad_len = d.seqs(t[:1], [PAGE * t.shape[1] + 1], [1])
+    bad_page = d.seqs(np.full((1, 2), d.n_pages, np.int32), [90], [1])
+    out = gpu.zeros(2, 1, 128, device="cuda")
+    other = gpu.cuda.Stream()
+    gpu.cuda.synchronize()
+
+    def report(stream):
+        try:
+            d.c.status(stream)
+            return ""
+        except fz.FurnaceError as e:
+            return str(e)
+
+    for delay in range(0, 200000, 400):  # cycles
+        d.c.read(bad_len, out[0].data_ptr(), None, 128, stream=d.stream())
+        with gpu.cuda.stream(other):
+            gpu.cuda._sleep(delay)
+        d.c.read(bad_page, out[1].data_ptr(), None, 128, stream=other.cuda_stream)
+        first = report(d.stream())
+        second = report(other.cuda_stream)
+        assert "lengths or rows" in first and "lengths or rows" not in second, (delay, first, second)
+        assert ("page number" in first) != ("page number" in second), (delay, first, second)
+    d.c.status(d.stream())
