@@ -1474,8 +1474,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
     // warpgroup's denominator goes by the maximum of its own last step, the sums by that of the last.
     if (ok) {
       const float m0 = sm.last[0][row], m1 = sm.last[1][row], top = fmaxf(m0, m1);
-      const float l = (m0 == -INFINITY ? 0.f : sm.l[0][row] * kq_exp2(m0 - top)) +
-                      (m1 == -INFINITY ? 0.f : sm.l[1][row] * kq_exp2(m1 - top));
+      // without a maximum l is 0, or a NaN: maxima pass over scores that are no numbers
+      const float l = (m0 == -INFINITY ? sm.l[0][row] : sm.l[0][row] * kq_exp2(m0 - top)) +
+                      (m1 == -INFINITY ? sm.l[1][row] : sm.l[1][row] * kq_exp2(m1 - top));
       float inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
       if (a.parts > 1) {
         inv = 1.f / KR_P;
@@ -1695,12 +1696,15 @@ __global__ void __launch_bounds__(KR_JOIN_THREADS) k_kvq8_join(const __grid_cons
 #pragma unroll 4
   for (uint32_t i = 0; i < a.parts; i++) {
     const float* p = slot + (uint64_t)i * kr_part_floats<HD>();
-    const float m = p[KR_M * HD + row];
-    if (m == -INFINITY) continue;  // nothing seen: its sums may not be there
+    const float m = p[KR_M * HD + row], l = p[KR_M * HD + KR_M + row];
+    if (m == -INFINITY) {  // its sums may not be there; l is 0 where the row saw nothing, else a NaN
+      den += l;
+      continue;
+    }
     const float f = kq_exp2(m - top);
     float x[DPL];
     kq_ldn<DPL>(p + row * HD + lane * DPL, x);
-    den = fmaf(f, p[KR_M * HD + KR_M + row], den);
+    den = fmaf(f, l, den);
 #pragma unroll
     for (int d = 0; d < DPL; d++) acc[d] = fmaf(f, x[d], acc[d]);
   }

@@ -1,5 +1,7 @@
 """Calls around the edges of the 8-bit paged KV cache."""
 
+import math
+
 import numpy as np
 import pytest
 
@@ -89,3 +91,60 @@ def test_status_keeps_what_another_stream_finds_meanwhile(gpu):
         assert "lengths or rows" in first and "lengths or rows" not in second, (delay, first, second)
         assert ("page number" in first) != ("page number" in second), (delay, first, second)
     d.c.status(d.stream())
+
+
+def _no_numbers(d, table, lens, news, q, bad, window=0, sinks=0):
+    """Attention where the key blocks of positions `bad` are NaN: rows that see
+    one are NaN, the others what they are without."""
+    q, got = d.attend(table, lens, news, q=q, **(dict(window=window, sinks=sinks) if window else {}))
+    n, new = lens[0], news[0]
+    pos = np.arange(n - new, n)
+    seen = np.arange(n)[None] <= pos[:, None]
+    if window:
+        seen &= (np.arange(n)[None] > pos[:, None] - window) | (np.arange(n)[None] < sinks)
+    hit = (seen & bad[None, :n]).any(-1) | np.isnan(q).any((1, 2))
+    assert np.isnan(got[hit]).all(), np.argwhere(~np.isnan(got[hit]).all((1, 2)))[:4]
+    for j in np.flatnonzero(~hit)[:: max(1, (~hit).sum() // 6)]:
+        want, tol = d.plain.attend(table[0], int(pos[j]) + 1, q[j:j + 1], window=window, sinks=sinks)
+        assert (np.abs(got[j] - want[0]) <= tol[0]).all(), j
+    return hit
+
+
+@pytest.mark.parametrize("new", [1, 3, 150, 900])
+@pytest.mark.parametrize("span", [(0, 16), (0, 640), (640, 1296), (1100, 1300)])
+def test_keys_that_are_no_numbers_reach_every_row_that_sees_them(gpu, new, span):
+    """In every form of the attention (single tokens, a few, prompts whose pages
+    are cut into parts), also where all that a row or a part sees is NaN: never
+    a result that leaves those positions out."""
+    d = Dev(24, 8, 2, 64, 1400)
+    n = 1300
+    t = d.table([n])
+    d.append(t, [n], [n])
+    blocks = np.arange(n) // 16
+    bad = (blocks >= span[0] // 16) & (blocks <= (span[1] - 1) // 16)
+    for b in np.unique(blocks[bad]):
+        d.scales[int(t[0, b // 4]) + d.first, :, 0, b % 4] = math.nan
+    q = d.rows(new, 8, fz.F32)
+    hit = _no_numbers(d, t, [n], [new], q, bad)
+    assert hit.all() or new == 900
+    _no_numbers(d, t, [n], [new], q, bad, window=90, sinks=3)
+    _no_numbers(d, t, [n], [new], q, bad, window=200)
+    short = min(new, 40)
+    _no_numbers(d, t[:, :1], [40], [short], d.rows(short, 8, fz.F32), bad)
+
+
+@pytest.mark.parametrize("new", [2, 150, 900])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_queries_that_are_no_numbers_give_none(gpu, new, value):
+    """A query with a NaN or an infinity has no softmax; the rows beside it are
+    as ever."""
+    d = Dev(24, 8, 2, 64, 1400)
+    t = d.table([1300])
+    d.append(t, [1300], [1300])
+    x, dev = d.rows(new, 8, fz.F32)
+    at = [0, new // 2, new - 1] if new > 2 else [1]
+    for j in at:
+        x[j] = math.nan  # what the check takes such a row for
+        dev[j, 5::64] = value
+    _no_numbers(d, t, [1300], [new], (x, dev), np.zeros(1300, bool))
+    _no_numbers(d, t, [1300], [new], (x, dev), np.zeros(1300, bool), window=100, sinks=2)
