@@ -462,12 +462,14 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // to the running sums in f32.
 //
 // Softmax: with scores x_t (base 2) and value scales v_t the running maximum m
-// is taken over x_t + log2 v_t.  The weights w_t = 2^(x_t - m) v_t that
-// multiply the codes are then at most 1, whatever the scales, and l = sum
-// 2^(x_t - m) is the denominator.  m follows that maximum only when it falls
-// behind by 2^8 (fp16 holds the weights up to there), so that the sums are
-// seldom rescaled.  Scales under 2^-100 count as that in m, so that l stays
-// finite.
+// is taken over x_t + log v_t, the logarithm rounded down to an integer.  The
+// weights w_t = 2^(x_t + log v_t - m) that multiply the codes, once the rest of
+// v_t is multiplied in, are then at most 2, whatever the scales, and l = sum w_t
+// 2^-log v_t is the denominator.  Its terms are found from the weights, not from
+// 2^(x_t - m): with scales near the end of f32's range that is no normal number.
+// m follows its maximum only when it falls behind by 2^8 (fp16 holds the weights
+// up to there), so that the sums are seldom rescaled.  Scales under 2^-96 count as
+// that in m, so that l stays finite.
 //
 // Measured with the merge: 16 sequences of 32768 positions, 8 KV heads of 128,
 // 64 query heads (1.08 GB) 188 us, 5.7 TB/s (220 us where calls follow each
@@ -483,7 +485,7 @@ constexpr uint32_t KQ_SP_POS = 32;       // positions of a page that a warp take
 constexpr float KQ_LAG = 8.f;            // m is at most this far behind (base 2)
 constexpr uint32_t KQ_SEG = 2;           // a segment's cost besides its pages, in pages
 constexpr uint32_t KQ_WHOLE_PAGES = 4;
-constexpr float KQ_MIN_SCALE = 7.8886090522101181e-31f;  // 2^-100
+constexpr float KQ_MIN_SCALE = 1.2621774483536189e-29f;  // 2^-96
 
 template <int HD>
 struct KqSplitSmem {
@@ -661,6 +663,19 @@ struct KqRows {
   }
 };
 
+// A block's value scale v as rest * 2^log, inv = 2^-log; log from -96 (v below
+// that: rest takes it, and 0) to 122.  For a v that is no number log is some number
+// and rest is v.
+struct KqScale {
+  float log, inv, rest;
+  __device__ __forceinline__ explicit KqScale(float v) {
+    const uint32_t e = __float_as_uint(fminf(fmaxf(v, KQ_MIN_SCALE), 5.316911983139664e36f)) >> 23;  // 31 .. 249
+    log = (float)((int)e - 127);
+    inv = __uint_as_float((254 - e) << 23);
+    rest = v * inv;
+  }
+};
+
 // Pages v0 .. v0 + nv - 1 of a segment.  The result goes to out where these
 // are all of its pages, else to the slot.  Called by the whole CTA.
 template <int HD, typename T>
@@ -770,9 +785,10 @@ __device__ __forceinline__ void kq_segment(const KqSplitArgs<HD, T>& a, KqSplitS
           }
         }
       }
-      const float va = st.vs[0], vb = st.vs[1];
-      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) + __log2f(fmaxf(va, KQ_MIN_SCALE)),
-                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) + __log2f(fmaxf(vb, KQ_MIN_SCALE)));
+      // each block's scale as (1 .. 2) times a power of two
+      const KqScale va(st.vs[0]), vb(st.vs[1]);
+      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) + va.log,
+                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) + vb.log);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       if (__any_sync(0xffffffffu, top > m + KQ_LAG)) {
@@ -782,14 +798,14 @@ __device__ __forceinline__ void kq_segment(const KqSplitArgs<HD, T>& a, KqSplitS
 #pragma unroll
         for (int n = 0; n < HD / 8; n++) o[n][0] *= f, o[n][1] *= f;
       }
-      const float sub_m = m == -INFINITY ? 0.f : m;
+      const float sub_m = m == -INFINITY ? 0.f : m, ca = va.log - sub_m, cb = vb.log - sub_m;
       float wv[8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float e = kq_exp2(x[k] - sub_m);
-        l += e;
-        wv[k] = e * (k < 4 ? va : vb);
-      }
+      for (int k = 0; k < 8; k++) wv[k] = kq_exp2(x[k] + (k < 4 ? ca : cb));
+      l = fmaf((wv[0] + wv[1]) + (wv[2] + wv[3]), va.inv, l);
+      l = fmaf((wv[4] + wv[5]) + (wv[6] + wv[7]), vb.inv, l);
+#pragma unroll
+      for (int k = 0; k < 8; k++) wv[k] *= k < 4 ? va.rest : vb.rest;
       if (hidden) {  // 0, whatever the scale of a block without positions of the sequence
 #pragma unroll
         for (int k = 0; k < 8; k++)
@@ -1076,7 +1092,7 @@ constexpr uint32_t KR_M = 128;
 constexpr uint32_t KR_THREADS = 512;
 constexpr uint32_t KR_CONV = 3;            // warps that convert keys
 constexpr uint32_t KR_POS = 2 * KQ_PAGE;   // positions of a step
-constexpr float KR_P = 8192.f;             // scale of the weights
+constexpr float KR_LOGP = 13.f;            // the weights are scaled by 2^13
 // registers: 128 a thread at launch, 512 for the four warpgroups together
 constexpr int KR_REG_ACC = 200, KR_REG_OTHER = 104;
 static_assert(3 * KR_REG_OTHER + KR_REG_ACC <= 512, "register shares");
@@ -1214,8 +1230,9 @@ __device__ __forceinline__ void kr_put(const float* x, uint32_t t) {
   kr_st8(t, hi);
   kr_st8(t + 16, lo);
 }
-// The block's weights 2^(f s - m) v KR_P: c = log2(v KR_P) - m puts the scale
-// into the exponent, and the denominator is the weights' sum / (v KR_P).
+// The block's weights 2^(f s - m) v 2^KR_LOGP: c = log2 v + KR_LOGP - m puts the
+// scales into the exponent.  Returns their sum, which divided by v is the
+// denominator's share, with the same 2^KR_LOGP as the sums have.
 __device__ __forceinline__ float kr_weights(float* x, float f, float c) {
   float2 sum[2] = {};
 #pragma unroll
@@ -1227,20 +1244,20 @@ __device__ __forceinline__ float kr_weights(float* x, float f, float c) {
   }
   return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
-// The same with positions that the row does not see, and for any scale: w = v
-// KR_P apart from the exponent.  Returns the denominator.
-__device__ __forceinline__ float kr_weights_masked(float* x, float f, float w, float m, uint32_t bits) {
+// The same with positions that the row does not see, and for any scale: v is the
+// block's, c goes by the larger of it and KQ_MIN_SCALE.
+__device__ __forceinline__ float kr_weights_masked(float* x, float f, float c, float v, uint32_t bits) {
+  const float less = v >= KQ_MIN_SCALE ? 1.f : v * (1.f / KQ_MIN_SCALE);  // a NaN stays one
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 16; k++) {
     const bool seen = bits >> k & 1;
-    const float e = kq_exp2(fmaf(x[k], f, -m));
-    sum += seen ? e : 0.f;
-    x[k] = seen ? e * w : 0.f;  // 0 whatever the scale of a block not written yet
+    const float w = kq_exp2(fmaf(x[k], f, c));
+    sum += seen ? w : 0.f;
+    x[k] = seen ? w * less : 0.f;  // 0 whatever the scale of a block not written yet
   }
   return sum;
 }
-
 template <int HD, typename T>
 __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_constant__ KqSplitArgs<HD, T> a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -1477,9 +1494,9 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
       // without a maximum l is 0, or a NaN: maxima pass over scores that are no numbers
       const float l = (m0 == -INFINITY ? sm.l[0][row] : sm.l[0][row] * kq_exp2(m0 - top)) +
                       (m1 == -INFINITY ? sm.l[1][row] : sm.l[1][row] * kq_exp2(m1 - top));
-      float inv = l == 0.f ? 0.f : __fdiv_rn(1.f / KR_P, l);
+      float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // 2^KR_LOGP is in the sums and in l
       if (a.parts > 1) {
-        inv = 1.f / KR_P;
+        inv = 1.f;
         slot[KR_M * HD + row] = top;
         slot[KR_M * HD + KR_M + row] = l;
       }
@@ -1649,13 +1666,14 @@ __global__ void __launch_bounds__(KR_THREADS, 1) k_kvq8_rows(const __grid_consta
         kr_ld32(t + 32 * j, x);
         kr_wait_ld(x);
         kr_wait_ld(x + 16);
-        if (!masked && fminf(v0, v1) >= KQ_MIN_SCALE) {
-          const float lp = 13.f - sub;  // log2 KR_P - m
-          l = fmaf(kr_weights(x, f0, a0 + lp), __fdividef(1.f / KR_P, v0), l);
-          l = fmaf(kr_weights(x + 16, f1, a1 + lp), __fdividef(1.f / KR_P, v1), l);
+        const float lp = KR_LOGP - sub;
+        if (!masked && v0 >= KQ_MIN_SCALE && v1 >= KQ_MIN_SCALE) {  // else the scales may be no numbers
+          l = fmaf(kr_weights(x, f0, a0 + lp), __fdividef(1.f, v0), l);
+          l = fmaf(kr_weights(x + 16, f1, a1 + lp), __fdividef(1.f, v1), l);
         } else {
           const uint32_t bits = masked ? vis(j) : 0xffffffffu;
-          l += kr_weights_masked(x, f0, v0 * KR_P, sub, bits) + kr_weights_masked(x + 16, f1, v1 * KR_P, sub, bits >> 16);
+          l = fmaf(kr_weights_masked(x, f0, a0 + lp, v0, bits), __fdividef(1.f, fmaxf(v0, KQ_MIN_SCALE)), l);
+          l = fmaf(kr_weights_masked(x + 16, f1, a1 + lp, v1, bits >> 16), __fdividef(1.f, fmaxf(v1, KQ_MIN_SCALE)), l);
         }
         kr_put(x, t + 32 * j);
         kr_put(x + 16, t + 32 * j + 8);

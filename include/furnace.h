@@ -390,10 +390,13 @@ int fz_kvq8_append_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype,
  * positions (append first): row at position p, query head h sees positions t
  * <= p of KV head h / (n_heads / n_kv_heads); with a window (0: none) only
  * those with t > p - window or t < sinks.  q is rotated at p like k.  out =
- * sum_t softmax(scale * q.k)_t v_t, statistics and sums in f32; scale 0 means
- * 1 / sqrt(head_dim).  out must not overlap q.  work: device scratch of at
- * least fz_kvq8_attend_work bytes, 16-byte aligned, contents don't matter;
- * calls that may run at the same time need one each. */
+ * sum_t softmax(scale * q.k)_t v_t, statistics and sums in f32: f32's precision
+ * for values from 1e-27 on (smaller ones may be off by 3e-38 a position) whose
+ * blocks' scales lie within 2^90 of each other in a sequence.  A score or value
+ * that is no number makes the rows that see it NaN.  scale 0 means 1 /
+ * sqrt(head_dim).  out must not overlap q.  work: device scratch of at least
+ * fz_kvq8_attend_work bytes, 16-byte aligned, contents don't matter; calls that
+ * may run at the same time need one each. */
 int fz_kvq8_attend_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, const void* q, uint64_t ldq,
                        void* out, uint64_t ldo, uint32_t window, uint32_t sinks, float scale, void* work,
                        uint64_t work_bytes, void* stream);

@@ -148,3 +148,69 @@ def test_queries_that_are_no_numbers_give_none(gpu, new, value):
         dev[j, 5::64] = value
     _no_numbers(d, t, [1300], [new], (x, dev), np.zeros(1300, bool))
     _no_numbers(d, t, [1300], [new], (x, dev), np.zeros(1300, bool), window=100, sinks=2)
+
+
+@pytest.mark.parametrize("new", [1, 5, 33, 130, 900])
+@pytest.mark.parametrize("spread", [3e33, 6e37])
+def test_values_up_to_the_end_of_the_range(gpu, new, spread):
+    """Values whose scales are far above 2^96, with scores that differ by many
+    powers of two: every form keeps the small weights, and nothing overflows
+    that the result does not."""
+    d = Dev(24, 8, 2, 64, 1400)
+    n = 1300
+    t = d.table([n])
+    k, v = d.rows(n, 2, fz.F32, spread=3.0), d.rows(n, 2, fz.F32)
+    v[0][:] = np.clip(v[0], -4, 4) * np.float32(spread)
+    v[1][:] = gpu.from_numpy(v[0].reshape(n, -1)).cuda()
+    d.append(t, [n], [n], k=k, v=v)
+    for kw in ({}, dict(window=300, sinks=5)):
+        d.check_attend(t, [n], [new], **kw)
+    short = min(new, 60)
+    d.check_attend(t[:, :1], [60], [short])
+
+
+@pytest.mark.parametrize("new", [1, 5, 130, 900])
+def test_value_scales_80_powers_of_two_apart(gpu, new):
+    """Blocks of tiny values between blocks of huge ones: their weights count in
+    the denominator all the same."""
+    d = Dev(24, 8, 2, 64, 1400)
+    n = 1280
+    t = d.table([n])
+    k, v = d.rows(n, 2, fz.F32, spread=2.0), d.rows(n, 2, fz.F32)
+    v[0][:] *= np.repeat(np.where(np.arange(n // 16) % 3 == 0, 2.0 ** 90, 2.0 ** 10), 16)[:, None, None].astype(np.float32)
+    v[1][:] = gpu.from_numpy(v[0].reshape(n, -1)).cuda()
+    d.append(t, [n], [n], k=k, v=v)
+    d.check_attend(t, [n], [new])
+    d.check_attend(t, [n], [new], window=200, sinks=20)
+
+
+@pytest.mark.parametrize("new", [1, 150, 900])
+@pytest.mark.parametrize("block", [0, 1, 34, 35, 81])
+def test_value_scales_that_are_no_numbers(gpu, new, block):
+    """One block of values without numbers, next to one with: the rows that see
+    it are NaN, the others as ever."""
+    d = Dev(24, 8, 2, 64, 1400)
+    n = 1300
+    t = d.table([n])
+    d.append(t, [n], [n])
+    d.scales[int(t[0, block // 4]) + d.first, :, 1, block % 4] = math.nan
+    bad = np.arange(n) // 16 == block
+    q = d.rows(new, 8, fz.F32)
+    _no_numbers(d, t, [n], [new], q, bad)
+    _no_numbers(d, t, [n], [new], q, bad, window=100, sinks=3)
+
+
+@pytest.mark.parametrize("new", [1, 130, 900])
+@pytest.mark.parametrize("spread", [1e-29, 1e-33, 0.0])
+def test_tiny_and_zero_values_over_many_positions(gpu, new, spread):
+    """Scales down to 2^-96 keep f32's precision; below that the two fp16 parts of
+    a weight, at most 1, end at 2^-36, and zeros stay zeros."""
+    d = Dev(24, 8, 2, 64, 1400)
+    n = 1300
+    t = d.table([n])
+    d.append(t, [n], [n], v=d.rows(n, 2, fz.F32, spread=spread))
+    q, got = d.attend(t, [n], [new])
+    want, tol = d.plain.attend(t[0], n, q)
+    # n weights off by half of 2^-35, codes up to 127, a denominator of 1 or more
+    assert (np.abs(got - want) <= tol + n * 127 * 2.0 ** -36 * 2.0 ** -96).all()
+    assert spread or not got.any()
