@@ -154,7 +154,9 @@ int fz_kv_new(fz_model* m, uint32_t max_ctx, int kv_dtype, fz_kv** out);
  * then accepts only fz_kv_free and fz_kv_len (the rest return FZ_EINVAL). */
 void fz_kv_free(fz_kv* kv);
 /* KvCache::len (src/model.rs:324).  set_len rewinds (or restores) the
- * filled length; positions >= len are overwritten by later forwards. */
+ * filled length; positions >= len are overwritten by later forwards.  An 8-bit
+ * cache rewound into a block of 16 keeps the block's scale: what the dropped
+ * positions did to it (a larger scale, a NaN) stays with the block's others. */
 int fz_kv_len(const fz_kv* kv, uint32_t* len);
 int fz_kv_set_len(fz_kv* kv, uint32_t len);
 /* kv.len = 0: the cache reused for a new sequence. */
@@ -380,9 +382,13 @@ typedef struct fz_kvq8_seqs {
  * every block written, scale = (largest magnitude of the call's values in it)
  * / 127, and at least the block's scale so far when it keeps older positions;
  * these then take the codes round(code * (old scale / scale)).  Codes are
- * round(x / scale), all in f32, rounding to nearest even.  Values must be
- * finite; one that is not makes the block's scale a NaN (reported).  Two
- * sequences of a call must not append to the same page. */
+ * round(x / scale), all in f32, rounding to nearest even.  So a value is off by
+ * at most half a code when it is appended, and by up to half a code of the
+ * block's last scale more for every later call that raises the scale: within 8
+ * codes (a block filled a position a call) whatever the values, half a code
+ * where whole blocks are appended.  Values must be finite; one that is not makes
+ * the block's scale a NaN (reported).  Two sequences of a call must not append
+ * to the same page. */
 int fz_kvq8_append_dev(const fz_kvq8* kv, const fz_kvq8_seqs* s, uint32_t dtype, const void* k, const void* v,
                        uint64_t ld, void* stream);
 
