@@ -42,11 +42,13 @@ struct OnDeviceOf {
 };
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 KvQ8Dev device_view(const fz_kvq8* kv) {
   need(kv != nullptr, "null cache");
   need(kv->codes && kv->scales && kv->status, "null cache buffer");
   need(aligned16(kv->codes) && aligned16(kv->scales), "codes and scales must be 16-byte aligned");
+  need(aligned4(kv->status), "the status word must be 4-byte aligned");
   need(kv->head_dim == 64 || kv->head_dim == 128, "head_dim %u unsupported (64 or 128)", kv->head_dim);
   need(kv->n_kv_heads > 0 && kv->n_kv_heads <= 65535, "%u KV heads unsupported", kv->n_kv_heads);
   need(kv->n_heads > 0 && kv->n_heads <= 65535 && kv->n_heads % kv->n_kv_heads == 0,
@@ -71,6 +73,8 @@ KvQ8Batch device_view(const fz_kvq8_seqs* s) {
   need(s->n_seqs <= 65535, "%u sequences in one call, the limit is 65535", s->n_seqs);
   if (s->n_seqs) {
     need(s->pages && s->lens, "null page table or lengths");
+    need(aligned4(s->pages) && aligned4(s->lens) && aligned4(s->starts),
+         "page table, lengths and row starts must be 4-byte aligned");
     need(s->max_pages > 0 && s->max_pages <= 0x7fffffffu / FZ_KVQ8_PAGE, "%u pages per sequence unsupported",
          s->max_pages);
     need(s->max_new > 0 && s->max_new <= s->max_pages * FZ_KVQ8_PAGE, "%u new positions do not fit %u pages",
