@@ -1885,6 +1885,10 @@ static void kvq8_attend_t(const KvQ8Attend& a, cudaStream_t s) {
 void launch_kvq8_attend(const KvQ8Attend& a, cudaStream_t s) {
   if (!a.b.n_seqs) return;
   if (a.runs && a.b.n_seqs * a.b.max_new != 1) fail(FZ_EINVAL, "run records are made for one row");
+  // With records every segment goes through the merge, and a run has two slots: as many runs as segments, so that none
+  // holds more than two of them (a run is then at most a page longer than a segment).
+  if (a.runs && a.c.nkv * ((a.c.group + 7) / 8) > kvq8_runs(a.c, a.b))
+    fail(FZ_EINVAL, "%u KV heads in a step on an 8-bit cache, the limit is %u", a.c.nkv, kvq8_runs(a.c, a.b));
   if (a.c.hd == 128)
     a.f16 ? kvq8_attend_t<128, __half>(a, s) : kvq8_attend_t<128, float>(a, s);
   else

@@ -60,3 +60,35 @@ def test_nothing_is_read_through_the_read_only_path():
     code = _code()
     assert "__ldg" not in code and ".nc" not in code
     assert not re.search(r"const [\w:]+\s*\*\s*__restrict__", code)
+
+
+def _slots(segments, pages, runs):
+    """(run, slot) of every piece that a step with run records writes, as
+    k_kvq8_split cuts them: a segment costs its pages and 2."""
+    size = pages + 2
+    total = segments * size
+    per = (total + 2 * runs - 1) // (2 * runs) * 2
+    out = []
+    for run in range(runs):
+        w0, w1 = min(per * run, total), min(per * run + per, total)
+        w = w0
+        while w < w1:
+            u0 = w % size
+            u1 = min(size, u0 + w1 - w)
+            if max(u1, 2) > max(u0, 2):
+                out.append((run, w != w0))
+            w += u1 - u0
+    return out
+
+
+def test_a_run_of_a_decode_step_has_room_for_its_pieces():
+    """As long as there are no more segments than runs; a step with more is
+    refused."""
+    assert len(_slots(900, 1, 444)) != len(set(_slots(900, 1, 444)))  # why it has to be
+    for segments in (1, 2, 7, 8, 64, 221, 222, 223, 300, 443, 444):
+        for pages in (1, 2, 3, 4, 5, 31, 32, 64, 1001):
+            runs = min(segments * (pages + 2), 444)
+            pieces = _slots(segments, pages, runs)
+            assert len(pieces) == len(set(pieces)), (segments, pages)
+    code = _code()
+    assert "a.runs && a.c.nkv * ((a.c.group + 7) / 8) > kvq8_runs(a.c, a.b)" in code
