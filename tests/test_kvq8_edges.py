@@ -214,3 +214,34 @@ def test_tiny_and_zero_values_over_many_positions(gpu, new, spread):
     # n weights off by half of 2^-35, codes up to 127, a denominator of 1 or more
     assert (np.abs(got - want) <= tol + n * 127 * 2.0 ** -36 * 2.0 ** -96).all()
     assert spread or not got.any()
+
+
+@pytest.mark.parametrize("hd, kv, group, dtype", [(128, 2, 7, fz.F32), (64, 1, 4, fz.F16)])
+def test_one_prompt_beside_single_tokens(gpu, hd, kv, group, dtype):
+    """What a serving step looks like: a prompt among sequences with a token
+    each, and idle ones; its rows, theirs and the cache are as in calls of their
+    own."""
+    lens = [700, 40, 0, 1033, 64, 1, 300, 0, 129]
+    d = Dev(60, kv * group, kv, hd, 1100)
+    t = d.table(lens)
+    news = [1, 1, 0, 1033, 1, 1, 1, 0, 1]
+    old = [n - new for n, new in zip(lens, news)]
+    d.append(t, old, old, dtype)
+    d.append(t, lens, news, dtype)
+    gpu.cuda.synchronize()
+    d.check_cache([(t[i], n) for i, n in enumerate(lens) if n])
+    d.check_attend(t, lens, news, dtype)
+    d.check_attend(t, lens, news, dtype, window=100, sinks=5)
+
+
+@pytest.mark.parametrize("new", [1, 12, 130])
+def test_a_table_much_wider_than_its_sequences(gpu, new):
+    """A table as wide as the longest sequence a server takes, and short
+    sequences: the entries past their ends are not read."""
+    lens = [130, 140, 1, 400]
+    d = Dev(20, 8, 2, 64, 500)
+    t = d.table(lens, spare=505)
+    d.append(t, lens, lens)
+    news = [min(new, n) for n in lens]
+    d.check_attend(t, lens, news)
+    d.check_attend(t, lens, news, window=70, sinks=2)
