@@ -472,9 +472,9 @@ __global__ void __launch_bounds__(HD) k_kvq8_read(KvQ8Dev c, KvQ8Batch b, T* __r
 // that in m, so that l stays finite.
 //
 // Measured with the merge: 16 sequences of 32768 positions, 8 KV heads of 128,
-// 64 query heads (1.08 GB) 188 us, 5.7 TB/s (220 us where calls follow each
+// 64 query heads (1.08 GB) 193 us, 5.6 TB/s (230 us where calls follow each
 // other for seconds: the power limit); 48 ragged ones of up to 8192, 4 KV heads
-// (208 MB) 49 us, of which about 5 pass before the first page has come and 3 in
+// (208 MB) 53 us, of which about 5 pass before the first page has come and 3 in
 // the merge.  Multiplies and sums in pairs took the last 2 %.  16 rows a segment,
 // or more runs than the SMs hold at once, are not faster.
 // ---------------------------------------------------------------------------
@@ -1759,7 +1759,7 @@ static void kvq8_append_t(const KvQ8Dev& c, const KvQ8Batch& b, const void* k, c
   });
   // one sequence: every SM filled once, a CTA taking as many items as that leaves it (8192 positions of 8 heads 20.4 us;
   // an item a CTA 23.0).  Several may be shorter than max_new: an item a CTA keeps the SMs even (ragged prompts 7 us;
-  // cut like one sequence 10)
+  // cut like one sequence 10), which two equal ones of 8192 pay for (41 us)
   const uint64_t items = (uint64_t)kvq8_blocks(b) * c.nkv, slots = (uint64_t)num_sms() * kq_ap_ctas<HD>();
   const uint64_t per = b.n_seqs > 1 ? 1 : (items + slots - 1) / slots;
   launch_pdl(k_kvq8_append<HD, T>, dim3((unsigned)((items + per - 1) / per), b.n_seqs), dim3(HD), sizeof(Stages), s, c,
@@ -1812,7 +1812,10 @@ static uint32_t kvq8_parts(const KvQ8Dev& c, const KvQ8Batch& b) {
 // the split form 2.8 ns with all SMs at work; starting and joining takes 17 and
 // 7.  Measured (us, split / rows): 1 sequence, 20 rows x 7 heads on 1000
 // positions 13.8 / 21.4, 100 rows on 2000 46 / 28, 512 rows on 3000 288 / 71;
-// 12 x 6 rows on up to 3000 37 / 63.
+// 12 x 6 rows x 5 heads on up to 3000 37 / 63, all on 3000 68 / 60.  The lengths
+// are on the device, so the table's width stands for them: a wide one with short
+// sequences goes to k_kvq8_rows (20 rows on 20 positions, 512 pages: 27 us, with
+// one page 8).
 static bool kvq8_by_rows(const KvQ8Dev& c, const KvQ8Batch& b) {
   const double pages = b.max_pages, groups = (double)b.n_seqs * c.nkv * (((uint64_t)b.max_new * c.group + 7) / 8);
   const double waves = std::ceil((double)kvq8_tiles(c, b) * c.nkv * b.n_seqs / num_sms());

@@ -365,7 +365,10 @@ typedef struct fz_kvq8 {
  * starts[i] (0 .. max_new) positions are rows starts[i] .. of the call's row
  * buffers; NULL: every sequence has max_new rows, i * max_new .., but one of
  * length 0 (an idle slot of a batch of fixed size) has none.  n_rows: the rows
- * the buffers hold (rows of no sequence are left as they are). */
+ * the buffers hold (rows of no sequence are left as they are).  The choice of
+ * kernels, their grids and the workspace go by max_pages and max_new, which the
+ * host knows: a table much wider than its sequences, or one long prompt beside
+ * single tokens, costs time, so narrow tables and a call for each kind are best. */
 typedef struct fz_kvq8_seqs {
   const int32_t* pages;
   const int32_t* lens;
